@@ -151,6 +151,61 @@ int qw35_cuda_gqa_decode_noalloc(uint32_t n_seq, const float *q, const float *ga
                                  uint64_t v_off, int32_t window, int32_t sink, float *out, void *stream, char *err,
                                  uintptr_t err_len);
 
+// Token runs and shared prefixes over the same cache ---------------------------
+// The three calls below take the same chunk tables, planes and head layout for
+// any number of tokens per sequence.  kv_type: 0 f16 planes, 1 q8_0 planes (as
+// kv_cache_type).  dtype: 0 f32, 1 f16, of q, gate and out.  All index arrays are
+// device memory, so the calls can be captured into a CUDA graph and replayed
+// over other lengths within the host's upper bounds.  q, gate and out are
+// [rows][16][256], 16-byte aligned, as is every chunk address.
+
+// Appends n_tok tokens to the cache: per-head RMS norm of q and k, rotary
+// positions on dims [0, 64) (NeoX pairs i, i + 32), K and V rows written for table
+// row tok_seq[t] at position tok_pos[t], q and gate out.  qkv [n_tok][qkv_stride]
+// as in qw35_cuda_attn_preprocess.  rope_pos [n_axes][n_tok]: rotary positions of
+// each token on 1 to 3 axes (time, height, width); sections [n_axes] (host): how
+// many of the 32 pairs turn by each axis, 32 in all (hparams.rope_sections).
+// interleaved 0: pairs [0, s0) by axis 0, the next s1 by axis 1, then axis 2.
+// interleaved 1 (three axes): pair i turns by axis i % 3 while i < 3 s_(i%3),
+// else by axis 0.  A token whose table row or position lies outside
+// [0, n_seq) x [0, 256 max_chunks), or whose table entry is 0, is padding:
+// nothing of it is written.  No two tokens may have the same row and position.
+int qw35_cuda_attn_append(uint32_t n_tok, const float *qkv, uint32_t qkv_stride, const float *q_norm_w,
+                          const float *k_norm_w, const float *rope_freq, const int32_t *rope_pos, uint32_t n_axes,
+                          const int32_t *sections, int interleaved, const int32_t *tok_seq, const int32_t *tok_pos,
+                          uint32_t n_seq, const uint64_t *chunk_ptrs, uint32_t max_chunks, uint64_t k_off,
+                          uint64_t v_off, uint32_t kv_type, void *q_out, void *gate_out, uint32_t dtype, float eps,
+                          void *stream, char *err, uintptr_t err_len);
+
+// Causal attention of ragged token runs: rows [run_off[i], run_off[i+1]) are the
+// last tokens of sequence i (table row i), whose context length with them is
+// seq_len[i]; the run's row t attends positions [0, seq_len[i] - run length + t],
+// cut by window and sink as in qw35_cuda_gqa_decode.  n_row is the number of rows
+// of q; rows outside every run are left as they were.  max_run and max_len are
+// upper bounds of a run's rows and of seq_len.  Cache rows within seq_len[i] have
+// to be finite; what lies behind them is not looked at.
+uint64_t qw35_cuda_gqa_prefill_workspace_bytes(uint32_t n_row, uint32_t n_run, uint32_t max_run, uint32_t max_len);
+int qw35_cuda_gqa_prefill(uint32_t n_row, const void *q, const void *gate, uint32_t dtype, uint32_t n_run,
+                          const int32_t *run_off, const int32_t *seq_len, uint32_t max_run, uint32_t max_len,
+                          const uint64_t *chunk_ptrs, uint32_t max_chunks, uint64_t k_off, uint64_t v_off,
+                          uint32_t kv_type, int32_t window, int32_t sink, void *out, void *workspace,
+                          uint64_t workspace_bytes, void *stream, char *err, uintptr_t err_len);
+
+// One decode step of sequences that share prefixes: what qw35_cuda_gqa_decode
+// computes for them, with each prefix read once per group.  Sequences
+// [group_off[g], group_off[g+1]) have the same keys and values at positions
+// [0, shared_len[g]) (read through the group's first table row); the rest of
+// their seq_len[i] positions are their own.  max_shared and max_own are upper
+// bounds of shared_len and of seq_len[i] - shared_len[g].
+uint64_t qw35_cuda_gqa_decode_shared_workspace_bytes(uint32_t n_seq, uint32_t n_group, uint32_t max_shared,
+                                                     uint32_t max_own);
+int qw35_cuda_gqa_decode_shared(uint32_t n_seq, const void *q, const void *gate, uint32_t dtype,
+                                const int32_t *seq_len, uint32_t n_group, const int32_t *group_off,
+                                const int32_t *shared_len, uint32_t max_shared, uint32_t max_own,
+                                const uint64_t *chunk_ptrs, uint32_t max_chunks, uint64_t k_off, uint64_t v_off,
+                                uint32_t kv_type, int32_t window, int32_t sink, void *out, void *workspace,
+                                uint64_t workspace_bytes, void *stream, char *err, uintptr_t err_len);
+
 // Batched runtime (extension of Qw35FFI.h) -----------------------------------
 // Sequences live in slots; slot 0 is the one the qw35_metal_* calls use.
 // Same arguments as qw35_metal_runtime_create plus the number of sequence

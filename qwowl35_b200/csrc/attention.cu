@@ -23,54 +23,18 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "kvcache.cuh"
 #include "ops.h"
 
 namespace qw35 {
 
-constexpr int AH = 16;      // query heads
-constexpr int AKV = 4;      // kv heads
-constexpr int AHD = 256;    // head dim
-constexpr int AGRP = AH / AKV;
-constexpr int ACHUNK = 256; // positions per chunk
 constexpr int ASPLIT = 256;  // positions per split (4 warps x 64): ~2 waves of CTAs at batch 32, ctx 4096
-constexpr int QFULL = AH * AHD * 2;  // q | gate per head
 constexpr int ASTG = 3;     // cp.async stages per warp in the split kernel (8 positions each)
 constexpr size_t ASMEM = (size_t)4 * ASTG * 2 * 8 * 32 * 16;  // 48 KiB of K/V staging per CTA
 // q8_0 planes: per warp a ring of raw q8_0 rows plus one dequantised f16 stage
 constexpr size_t ARAWQ8 = (size_t)ASTG * 2 * 8 * kKvQ8Row;             // 13,056 B
 constexpr size_t AQ8D = 16 * 8 * 4;                                     // block scales [16 rows][8 blocks] f32
 constexpr size_t ASMEM_Q8 = (size_t)4 * (ARAWQ8 + 2 * 8 * 32 * 16 + AQ8D);  // 87,040 B
-
-// One q8_0 block of 32 values held 8 per lane by 4 consecutive lanes (lane % 4
-// = the lane's quarter): qw35_q8_0_quantize_block (qw35_attention.metal:429-440).
-// d = amax / 127 in fp32, codes round(x * (1 / d)) (half away from zero)
-// clamped to +-127 with the fp32 d, the block stores half(d).  `blk` points at
-// the block's 34 bytes {f16 d; int8 qs[32]}; every lane of the warp calls this.
-__device__ __forceinline__ void q8_block_store(const float *x, uint8_t *blk, int lane) {
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const float d = amax / 127.0f;
-    const float id = d != 0.0f ? 1.0f / d : 0.0f;
-    uint32_t packed[2] = {0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = __fmul_rn(x[i], id);  // a plain product, as the reference (no contraction)
-        int q = (int)roundf(y);
-        q = q < -127 ? -127 : (q > 127 ? 127 : q);
-        packed[i >> 2] |= ((uint32_t)q & 0xffu) << (8 * (i & 3));
-    }
-    // the block starts 2 bytes before the codes; codes of quarter j at 2 + 8 j:
-    // even addresses, so 16-bit stores
-    unsigned short *qd = reinterpret_cast<unsigned short *>(blk + 2 + 8 * (lane & 3));
-    qd[0] = (unsigned short)(packed[0] & 0xffffu);
-    qd[1] = (unsigned short)(packed[0] >> 16);
-    qd[2] = (unsigned short)(packed[1] & 0xffffu);
-    qd[3] = (unsigned short)(packed[1] >> 16);
-    if ((lane & 3) == 0) *reinterpret_cast<unsigned short *>(blk) = __half_as_ushort(__float2half_rn(d));
-}
 
 // ---- preprocess: RMS norm + NeoX RoPE + f16 (or q8_0) KV write ----------------
 // One warp per head row (16 q heads + 4 kv heads = 20 warps): every row's
@@ -172,15 +136,6 @@ __device__ __forceinline__ void h8_to_f(const uint4 &u, float *f) {
 struct SplitPart {  // per (seq, head, split): m, l then acc[256] in a separate array
     float m, l;
 };
-
-__device__ __forceinline__ void attended_range(int L, int window, int sink, int &total, int &sk, int &rstart) {
-    sk = max(0, min(sink, L));
-    if (window <= 0 || sk + window >= L) {
-        sk = 0; rstart = 0; total = L;
-    } else {
-        rstart = L - window; total = sk + window;
-    }
-}
 
 // m16n8k16 f16 x f16 -> f32 (legacy warp MMA; this kernel is bound by HBM, the
 // tensor cores only retire its arithmetic)

@@ -294,4 +294,140 @@ int qw35_cuda_gqa_decode_noalloc(uint32_t n_seq, const float *q, const float *ga
     return cuda_ok(qw35::attn_decode_noalloc_run(a, (cudaStream_t)stream), "gqa_decode_noalloc", err, err_len);
 }
 
+// ---- token runs and shared prefixes ----------------------------------------------
+
+// Axis of each rotary pair, 2 bits a pair; false when the sections do not cover 32 pairs.
+static bool axis_map(uint32_t n_axes, const int32_t *sections, int interleaved, uint64_t *map) {
+    int64_t sum = 0;
+    for (uint32_t a = 0; a < n_axes; ++a) {
+        if (sections[a] < 0) return false;
+        sum += sections[a];
+    }
+    if (sum != 32) return false;
+    uint64_t m = 0;
+    for (int i = 0; i < 32; ++i) {
+        uint64_t axis = 0;
+        if (interleaved) {
+            const int a = i % 3;
+            axis = (a && i < 3 * sections[a]) ? (uint64_t)a : 0u;
+        } else {
+            int end = sections[0];
+            while (i >= end) end += sections[++axis];
+        }
+        m |= axis << (2 * i);
+    }
+    *map = m;
+    return true;
+}
+
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+
+int qw35_cuda_attn_append(uint32_t n_tok, const float *qkv, uint32_t qkv_stride, const float *q_norm_w,
+                          const float *k_norm_w, const float *rope_freq, const int32_t *rope_pos, uint32_t n_axes,
+                          const int32_t *sections, int interleaved, const int32_t *tok_seq, const int32_t *tok_pos,
+                          uint32_t n_seq, const uint64_t *chunk_ptrs, uint32_t max_chunks, uint64_t k_off,
+                          uint64_t v_off, uint32_t kv_type, void *q_out, void *gate_out, uint32_t dtype, float eps,
+                          void *stream, char *err, uintptr_t err_len) {
+    if (n_tok == 0) return 1;
+    if (!qkv || !q_norm_w || !k_norm_w || !rope_freq || !rope_pos || !sections || !tok_seq || !tok_pos || !chunk_ptrs ||
+        !q_out || !gate_out || qkv_stride < 10240 || n_seq == 0 || n_seq > (1u << 30) || max_chunks == 0 ||
+        max_chunks > (1u << 22) || n_tok > (1u << 30) || (k_off % 16) || (v_off % 16) || kv_type > 1 || dtype > 1 ||
+        !aligned16(q_out) || !aligned16(gate_out)) {
+        set_err(err, err_len, "invalid append arguments%s", "");
+        return 0;
+    }
+    qw35::AttnAppendArgs a;
+    if (n_axes < 1 || n_axes > 3 || (interleaved && n_axes == 2) ||
+        !axis_map(n_axes, sections, interleaved && n_axes == 3, &a.axis_map)) {
+        set_err(err, err_len,
+                "rotary sections must be 1 to 3 non-negative counts of 32 pairs in all (interleaved: 1 or 3)%s", "");
+        return 0;
+    }
+    a.n_tok = (int)n_tok; a.qkv = qkv; a.qkv_stride = (long long)qkv_stride; a.q_norm_w = q_norm_w;
+    a.k_norm_w = k_norm_w; a.rope_freq = rope_freq; a.rope_pos = rope_pos; a.tok_seq = tok_seq; a.tok_pos = tok_pos;
+    a.chunk_ptrs = chunk_ptrs; a.n_seq = (int)n_seq; a.max_chunks = (int)max_chunks; a.k_off = (long long)k_off;
+    a.v_off = (long long)v_off; a.q_out = q_out; a.gate_out = gate_out; a.half = (int)dtype; a.eps = eps;
+    a.kv_q8 = (int)kv_type;
+    return cuda_ok(qw35::attn_append_run(a, (cudaStream_t)stream), "attn_append", err, err_len);
+}
+
+// The checks that gqa_prefill and gqa_decode_shared have in common; fills `a`.
+static bool tile_args(qw35::AttnTileArgs &a, uint32_t n_row, const void *q, const void *gate, uint32_t dtype,
+                      uint32_t n_run, const int32_t *off, const int32_t *len, uint64_t max_pos,
+                      const uint64_t *chunk_ptrs, uint32_t max_chunks, uint64_t k_off, uint64_t v_off, uint32_t kv_type,
+                      int32_t window, int32_t sink, void *out, void *ws, uint64_t ws_bytes) {
+    if (!q || !off || !len || !chunk_ptrs || !out || !ws || n_run == 0 || max_chunks == 0 || max_chunks > (1u << 22) ||
+        (uint64_t)max_chunks * QW35_KV_CHUNK < max_pos || (k_off % 16) || (v_off % 16) || kv_type > 1 || dtype > 1 ||
+        !aligned16(q) || !aligned16(gate) || !aligned16(out) || !aligned16(ws))
+        return false;
+    a.n_row = (int)n_row; a.n_run = (int)n_run; a.q = q; a.gate = gate; a.out = out; a.half = (int)dtype;
+    a.off = off; a.len = len; a.chunk_ptrs = chunk_ptrs; a.max_chunks = (int)max_chunks;
+    a.k_off = (long long)k_off; a.v_off = (long long)v_off; a.kv_q8 = (int)kv_type;
+    a.window = window < 0 ? 0 : (window > (1 << 30) ? 1 << 30 : window);
+    a.sink = sink < 0 ? 0 : (sink > (1 << 30) ? 1 << 30 : sink);
+    a.ws = ws; a.ws_bytes = ws_bytes;
+    return true;
+}
+
+// Limits of the size queries too: rows and runs within a grid, lengths within the table's.
+static bool tile_sizes_ok(uint32_t n_row, uint32_t n_run, uint64_t len) {
+    return n_row <= (1u << 24) && n_run <= 65535 && len <= (1u << 30);
+}
+
+uint64_t qw35_cuda_gqa_prefill_workspace_bytes(uint32_t n_row, uint32_t n_run, uint32_t max_run, uint32_t max_len) {
+    if (!tile_sizes_ok(n_row, n_run, max_len)) return 0;
+    return qw35::attn_tile_workspace_bytes((int)n_row, (int)n_run, (int)max_run, (int)max_len, 0);
+}
+
+int qw35_cuda_gqa_prefill(uint32_t n_row, const void *q, const void *gate, uint32_t dtype, uint32_t n_run,
+                          const int32_t *run_off, const int32_t *seq_len, uint32_t max_run, uint32_t max_len,
+                          const uint64_t *chunk_ptrs, uint32_t max_chunks, uint64_t k_off, uint64_t v_off,
+                          uint32_t kv_type, int32_t window, int32_t sink, void *out, void *workspace,
+                          uint64_t workspace_bytes, void *stream, char *err, uintptr_t err_len) {
+    if (n_row == 0 || n_run == 0) return 1;
+    qw35::AttnTileArgs a;
+    if (max_run == 0 || max_run > n_row || max_len == 0 || !tile_sizes_ok(n_row, n_run, max_len) ||
+        !tile_args(a, n_row, q, gate, dtype, n_run, run_off, seq_len, max_len, chunk_ptrs, max_chunks, k_off, v_off,
+                   kv_type, window, sink, out, workspace, workspace_bytes)) {
+        set_err(err, err_len, "invalid prefill attention arguments%s", "");
+        return 0;
+    }
+    if (workspace_bytes < qw35_cuda_gqa_prefill_workspace_bytes(n_row, n_run, max_run, max_len)) {
+        set_err(err, err_len, "prefill attention workspace too small%s", "");
+        return 0;
+    }
+    a.max_run = (int)max_run; a.max_len = (int)max_len;
+    return cuda_ok(qw35::attn_tile_run(a, (cudaStream_t)stream), "gqa_prefill", err, err_len);
+}
+
+uint64_t qw35_cuda_gqa_decode_shared_workspace_bytes(uint32_t n_seq, uint32_t n_group, uint32_t max_shared,
+                                                     uint32_t max_own) {
+    if (!tile_sizes_ok(n_seq, n_group, max_shared) || !tile_sizes_ok(n_seq, n_group, max_own)) return 0;
+    return qw35::attn_tile_workspace_bytes((int)n_seq, (int)n_group, 0, (int)max_shared, (int)max_own);
+}
+
+int qw35_cuda_gqa_decode_shared(uint32_t n_seq, const void *q, const void *gate, uint32_t dtype,
+                                const int32_t *seq_len, uint32_t n_group, const int32_t *group_off,
+                                const int32_t *shared_len, uint32_t max_shared, uint32_t max_own,
+                                const uint64_t *chunk_ptrs, uint32_t max_chunks, uint64_t k_off, uint64_t v_off,
+                                uint32_t kv_type, int32_t window, int32_t sink, void *out, void *workspace,
+                                uint64_t workspace_bytes, void *stream, char *err, uintptr_t err_len) {
+    if (n_seq == 0 || n_group == 0) return 1;
+    qw35::AttnTileArgs a;
+    // (the longest prefix and the longest tail may belong to different groups)
+    const uint64_t longest = max_shared > max_own ? max_shared : max_own;
+    if (!shared_len || longest == 0 || n_seq > 65535 || !tile_sizes_ok(n_seq, n_group, longest) ||
+        !tile_args(a, n_seq, q, gate, dtype, n_group, group_off, seq_len, longest, chunk_ptrs, max_chunks, k_off, v_off,
+                   kv_type, window, sink, out, workspace, workspace_bytes)) {
+        set_err(err, err_len, "invalid shared-prefix attention arguments%s", "");
+        return 0;
+    }
+    if (workspace_bytes < qw35_cuda_gqa_decode_shared_workspace_bytes(n_seq, n_group, max_shared, max_own)) {
+        set_err(err, err_len, "shared-prefix attention workspace too small%s", "");
+        return 0;
+    }
+    a.shared_len = shared_len; a.max_len = (int)max_shared; a.max_own = (int)max_own;
+    return cuda_ok(qw35::attn_tile_run(a, (cudaStream_t)stream), "gqa_decode_shared", err, err_len);
+}
+
 }  // extern "C"

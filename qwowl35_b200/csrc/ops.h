@@ -129,6 +129,52 @@ cudaError_t attn_decode_run(const AttnArgs &a, cudaStream_t st);
 size_t attn_noalloc_limit();
 cudaError_t attn_decode_noalloc_run(AttnArgs a, cudaStream_t st);  // ws taken from a static device array
 
+// Token runs into the paged cache (attn_append.cu).
+struct AttnAppendArgs {
+    int n_tok = 0;
+    const float *qkv = nullptr;    // [n_tok][stride]: q_full(16*512) | k(1024) | v(1024)
+    long long qkv_stride = 0;
+    const float *q_norm_w = nullptr, *k_norm_w = nullptr;  // [256]
+    const float *rope_freq = nullptr;                      // [32]
+    const int32_t *rope_pos = nullptr;                     // [axes][n_tok]
+    uint64_t axis_map = 0;                                 // axis of pair i at bits 2i, 2i + 1
+    const int32_t *tok_seq = nullptr, *tok_pos = nullptr;  // [n_tok] chunk-table row (< 0: padding), cache position
+    const uint64_t *chunk_ptrs = nullptr;                  // [n_seq][max_chunks]
+    int n_seq = 0, max_chunks = 0;
+    long long k_off = 0, v_off = 0;
+    void *q_out = nullptr, *gate_out = nullptr;            // [n_tok][16][256], f32 or f16
+    int half = 0;                                          // 1: q_out and gate_out are f16
+    float eps = 1e-6f;
+    int kv_q8 = 0;
+};
+cudaError_t attn_append_run(const AttnAppendArgs &a, cudaStream_t st);
+
+// Attention of many rows over one stretch of the cache (attn_tile.cu): rows
+// [off[u], off[u+1]) are run u's tokens (shared_len null: causal, len[u] = the
+// run's context length after its last token, table row u), or group u's
+// sequences (shared_len[u] = their common prefix, len[r] = the context length of
+// sequence r, table row r).
+struct AttnTileArgs {
+    int n_row = 0, n_run = 0;
+    const void *q = nullptr, *gate = nullptr;  // [n_row][16][256], f32 or f16; gate may be null
+    void *out = nullptr;                       // [n_row][16][256], as q
+    int half = 0;
+    const int32_t *off = nullptr, *len = nullptr, *shared_len = nullptr;
+    int max_run = 0;               // upper bound of a run's rows (0: not known)
+    int max_len = 0;               // upper bound of a run's len / a group's shared_len
+    int max_own = 0;               // upper bound of len - shared_len
+    const uint64_t *chunk_ptrs = nullptr;
+    int max_chunks = 0;
+    long long k_off = 0, v_off = 0;
+    int window = 0, sink = 0;
+    float scale = 0.0625f;
+    void *ws = nullptr;
+    size_t ws_bytes = 0;
+    int kv_q8 = 0;
+};
+size_t attn_tile_workspace_bytes(int n_row, int n_run, int max_run, int max_len, int max_own);
+cudaError_t attn_tile_run(const AttnTileArgs &a, cudaStream_t st);
+
 unsigned int device_error_read_and_clear();
 
 cudaError_t rms_norm_run(const float *x, const float *w, float *out, int n, int k, float eps, cudaStream_t st);

@@ -6,6 +6,8 @@ stream.  There is no torch or CPU implementation behind any of them.
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 
 from ._lib import call, lib
@@ -141,4 +143,109 @@ def gqa_decode(q, gate, seq_len, max_len, chunk_ptrs, k_off, v_off, window=0, si
         ws = gqa_workspace(n, max_len, q.device)
     call("qw35_cuda_gqa_decode_q8_0" if kv_q8 else "qw35_cuda_gqa_decode", n, _p(_dev(q)), _p(gate), _p(_dev(seq_len)), max_len, _p(_dev(chunk_ptrs)),
          chunk_ptrs.shape[1], k_off, v_off, window, sink, _p(out), _p(ws), ws.numel(), _stream())
+    return out
+
+
+def _ints(t, *shape):
+    """A device int32 index array of the given shape."""
+    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+        raise TypeError(f"int32 tensor of shape {shape} expected, got {t.dtype} {tuple(t.shape)}")
+    return _p(_dev(t))
+
+
+def _table(t):
+    """A device chunk table [rows, chunks] of 64-bit addresses."""
+    if t.dtype not in (torch.int64, torch.uint64) or t.dim() != 2:
+        raise TypeError("chunk_ptrs must be a 2-d tensor of 64-bit addresses")
+    return _p(_dev(t))
+
+
+def _heads(t, n, dtype):
+    """q, gate or out: [n, 16, 256] (or [n, 4096]) values of `dtype`; None passes."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() != n * 4096:
+        raise TypeError(f"{dtype} tensor of {n} x 16 x 256 values expected, got {t.dtype} {tuple(t.shape)}")
+    return _p(_dev(t))
+
+
+def attn_append(qkv, q_norm_w, k_norm_w, rope_freq, rope_pos, sections, tok_seq, tok_pos, chunk_ptrs, k_off, v_off,
+                eps=1e-6, interleaved=True, dtype=torch.float32, kv_q8=False, q=None, gate=None):
+    """Append token runs to the cache; returns q and gate [n, 16, 256] as `dtype` (f32 or f16).
+
+    qkv [n, >= 10240] f32 (rows may be strided); rope_pos [axes, n] int32 rotary positions, `sections` the pairs per
+    axis; tok_seq / tok_pos [n] int32: chunk-table row (negative: padding, nothing written) and cache position.
+    """
+    n = qkv.shape[0]
+    if qkv.dtype != torch.float32 or not qkv.is_cuda or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < 10240:
+        raise TypeError("qkv must be a float32 device tensor [n, >= 10240] with contiguous rows")
+    for w, size in ((q_norm_w, 256), (k_norm_w, 256), (rope_freq, 32)):
+        if w.dtype != torch.float32 or w.numel() != size:
+            raise TypeError("norm weights (256) and rope_freq (32) must be float32")
+    q = torch.empty((n, 16, 256), dtype=dtype, device=qkv.device) if q is None else q
+    gate = torch.empty((n, 16, 256), dtype=dtype, device=qkv.device) if gate is None else gate
+    sec = (C.c_int32 * len(sections))(*sections)
+    call("qw35_cuda_attn_append", n, _p(qkv), qkv.stride(0) if n > 1 else qkv.shape[1], _p(_dev(q_norm_w)),
+         _p(_dev(k_norm_w)), _p(_dev(rope_freq)), _ints(rope_pos, len(sections), n), len(sections), sec,
+         1 if interleaved else 0, _ints(tok_seq, n), _ints(tok_pos, n), chunk_ptrs.shape[0], _table(chunk_ptrs),
+         chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0, _heads(q, n, dtype), _heads(gate, n, dtype),
+         _head_dtype(dtype), float(eps), _stream())
+    return q, gate
+
+
+def _head_dtype(dtype):
+    if dtype == torch.float32:
+        return 0
+    if dtype == torch.float16:
+        return 1
+    raise TypeError("q, gate and out must be float32 or float16")
+
+
+def gqa_prefill_workspace(n_row: int, n_run: int, max_run: int, max_len: int, device="cuda"):
+    n = int(lib().qw35_cuda_gqa_prefill_workspace_bytes(n_row, n_run, max_run, max_len))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def gqa_prefill(q, gate, run_off, seq_len, max_run, max_len, chunk_ptrs, k_off, v_off, window=0, sink=0, ws=None,
+                out=None, kv_q8=False):
+    """Causal attention of token runs over the cache that already holds them; [n, 4096] in q's type.
+
+    run_off [runs + 1], seq_len [runs] int32: rows run_off[i]..run_off[i+1] of q are the last tokens of sequence i.
+    """
+    n, runs = q.shape[0], seq_len.numel()
+    if chunk_ptrs.shape[0] < runs:
+        raise ValueError("chunk_ptrs needs a row for every run")
+    if out is None:
+        out = torch.empty((n, 4096), dtype=q.dtype, device=q.device)
+    if ws is None:
+        ws = gqa_prefill_workspace(n, runs, max_run, max_len, q.device)
+    call("qw35_cuda_gqa_prefill", n, _heads(q, n, q.dtype), _heads(gate, n, q.dtype), _head_dtype(q.dtype), runs,
+         _ints(run_off, runs + 1), _ints(seq_len, runs), max_run, max_len, _table(chunk_ptrs), chunk_ptrs.shape[1],
+         k_off, v_off, 1 if kv_q8 else 0, window, sink, _heads(out, n, q.dtype), _p(ws), ws.numel(), _stream())
+    return out
+
+
+def gqa_decode_shared_workspace(n_seq: int, n_group: int, max_shared: int, max_own: int, device="cuda"):
+    n = int(lib().qw35_cuda_gqa_decode_shared_workspace_bytes(n_seq, n_group, max_shared, max_own))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def gqa_decode_shared(q, gate, seq_len, group_off, shared_len, max_shared, max_own, chunk_ptrs, k_off, v_off, window=0,
+                      sink=0, ws=None, out=None, kv_q8=False):
+    """gqa_decode for sequences that share prefixes, each prefix read once per group; [n, 4096] in q's type.
+
+    group_off [groups + 1], shared_len [groups] int32: sequences group_off[g]..group_off[g+1] agree on their first
+    shared_len[g] positions.  max_shared, max_own: upper bounds of shared_len and of seq_len - shared_len.
+    """
+    n, groups = q.shape[0], shared_len.numel()
+    if chunk_ptrs.shape[0] < n:
+        raise ValueError("chunk_ptrs needs a row for every sequence")
+    if out is None:
+        out = torch.empty((n, 4096), dtype=q.dtype, device=q.device)
+    if ws is None:
+        ws = gqa_decode_shared_workspace(n, groups, max_shared, max_own, q.device)
+    call("qw35_cuda_gqa_decode_shared", n, _heads(q, n, q.dtype), _heads(gate, n, q.dtype), _head_dtype(q.dtype),
+         _ints(seq_len, n), groups, _ints(group_off, groups + 1), _ints(shared_len, groups), max_shared, max_own,
+         _table(chunk_ptrs), chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0, window, sink,
+         _heads(out, n, q.dtype), _p(ws), ws.numel(), _stream())
     return out

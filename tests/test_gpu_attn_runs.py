@@ -1,0 +1,614 @@
+"""Token runs and shared prefixes over the paged KV cache: append, run (prefill)
+attention and shared-prefix decode against plain 64-bit implementations.
+
+Bounds on an attention output o = sum p v / sum p, elementwise, with
+A = sum p |v| / sum p and S = max_j sum_i |q_i k_ij| / 16 of the row:
+  f32   q and p enter the tensor cores as f16 hi + lo (2^-22 relative each) and
+        products accumulate in chains of at most 32 steps per score (2^-23 of S a
+        step, truncated) and (positions / 8 + 64) steps per output:
+        |ds| <= 2^-17 S, |do| <= 2 |ds| A + (n / 8 + 64) 2^-23 A.
+  f16   besides that, p is rounded to f16 once (2^-11 A) and the result once
+        (2^-11 |o|).
+  f16 over q8_0 planes: K and V values d * q are rounded to f16 too:
+        |ds| += 2^-11 S, |do| += 2^-11 A.
+The sigmoid gate (at most 1) multiplies all of it, with 2^-22 |o| of its own.
+"""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from qwowl35_b200 import _lib
+
+H, KV, D, CH = 16, 4, 256, 256
+Q8ROW = 272
+EPS = 1e-6
+
+
+# ---- a cache and its plain reading -------------------------------------------------------
+
+class Cache:
+    """Shuffled chunks of two layers (the second is the one in use); everything unwritten is NaN (q8_0: NaN scales)."""
+
+    def __init__(self, lengths, q8, seed, max_chunks=None):
+        self.q8 = q8
+        self.plane = KV * CH * (Q8ROW if q8 else 2 * D)
+        self.k_off, self.v_off = 2 * self.plane, 3 * self.plane
+        counts = [-(-n // CH) for n in lengths]
+        g = torch.Generator().manual_seed(seed)
+        perm = torch.randperm(max(1, sum(counts)), generator=g)
+        self.raw = torch.zeros(max(1, sum(counts)), 4, self.plane, dtype=torch.uint8, device="cuda")
+        if q8:
+            self.raw.view(-1, 34)[:, :2] = torch.tensor([0, 0x7e], dtype=torch.uint8, device="cuda")
+        else:
+            self.raw.view(torch.float16).fill_(float("nan"))
+        self.ids = torch.full((len(lengths), max_chunks or max(1, max(counts))), -1, dtype=torch.int64)
+        at = 0
+        for i, c in enumerate(counts):
+            self.ids[i, :c] = perm[at:at + c]
+            at += c
+
+    def ptrs(self):
+        """The chunk table; entries that no chunk backs are 0."""
+        t = self.raw.data_ptr() + self.ids * 4 * self.plane
+        return torch.where(self.ids >= 0, t, torch.zeros_like(t)).cuda()
+
+    def rows(self):
+        """The layer's planes as [chunk, K or V, head, position, row]: f16 values, or q8_0 bytes [8, 34]."""
+        part = self.raw[:, 2:]
+        if self.q8:
+            return part.view(-1, 2, KV, CH, 8, 34)
+        return part.view(torch.float16).view(-1, 2, KV, CH, D)
+
+    def values(self):
+        """What the planes stand for, in 64 bits."""
+        r = self.rows()
+        if self.q8:
+            return (r[..., 2:].view(torch.int8).double() * r[..., :2].view(torch.float16).double()).flatten(-2)
+        return r.double()
+
+    def fill(self, lengths, seed, scale=1.0):
+        """Random rows at positions [0, lengths[i]) of every sequence."""
+        g = torch.Generator("cuda").manual_seed(seed)
+        rows = self.rows()
+        for i, n in enumerate(lengths):
+            for c in range(-(-n // CH)):
+                m = min(CH, n - c * CH)
+                part = rows[int(self.ids[i, c])][:, :, :m]
+                if self.q8:
+                    part[..., 2:] = torch.randint(-127, 128, part.shape[:-1] + (32,), dtype=torch.int8, device="cuda",
+                                                  generator=g).view(torch.uint8)
+                    d = (0.5 + torch.rand(part.shape[:-1] + (1,), device="cuda", generator=g)) * scale * 1.7 / 127
+                    part[..., :2] = d.half().view(torch.uint8)
+                else:
+                    part.copy_(torch.randn(part.shape, device="cuda", generator=g) * scale)
+        return self
+
+    def sequence(self, i, n):
+        """K, V [head, n, dim] of sequence i in 64 bits."""
+        v = self.values()[self.ids[i, :-(-n // CH)].cuda()] if n else self.values()[:0]
+        kv = v.permute(1, 2, 0, 3, 4).reshape(2, KV, -1, D)[:, :, :n]
+        return kv[0], kv[1]
+
+
+def attend(q, gate, k, v, length, window=0, sink=0):
+    """One row: q, gate [16, 256] -> (o, A, S) of the formulas above, 64 bits."""
+    q = q.double().view(KV, H // KV, D)
+    j = torch.arange(k.shape[1], device="cuda")
+    keep = j < length
+    few = min(sink, max(length, 0))
+    if window > 0 and few + window < length:
+        keep &= (j < few) | (j >= length - window)
+    sig = torch.sigmoid(gate.double()) if gate is not None else torch.ones(H, D, device="cuda", dtype=torch.float64)
+    if not bool(keep.any()):
+        z = torch.zeros(H, D, dtype=torch.float64, device="cuda")
+        return z, z, torch.zeros(H, 1, dtype=torch.float64, device="cuda")
+    k, v = k[:, keep], v[:, keep]
+    s = q @ k.transpose(1, 2) / math.sqrt(D)
+    p = torch.softmax(s, -1)
+    big = (q.abs() @ k.abs().transpose(1, 2)).amax(-1) / math.sqrt(D)
+    return (p @ v).view(H, D) * sig, (p @ v.abs()).view(H, D) * sig, big.view(H, 1)
+
+
+def bound(o, a, s, n, half, q8):
+    ds = 2.0 ** -17 * s
+    extra = (n / 8 + 64) * 2.0 ** -23 * a + 2.0 ** -22 * o.abs()
+    if half:
+        extra = extra + 2.0 ** -11 * a + 2.0 ** -11 * o.abs() + 2.0 ** -24
+        if q8:
+            ds = ds + 2.0 ** -11 * s
+            extra = extra + 2.0 ** -11 * a
+    return torch.expm1(2 * ds) * a + extra + 1e-30
+
+
+def check_rows(out, rows, half, q8):
+    """rows: [(row of out, o, A, S, context length)]."""
+    worst = 0.0
+    for r, o, a, s, n in rows:
+        y = out[r].double().view(H, D)
+        assert torch.isfinite(y).all(), r
+        worst = max(worst, float(((y - o).abs() / bound(o, a, s, max(n, 0), half, q8)).max()))
+    assert worst <= 1.0, worst
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def some(n, seed, kind, scale=1.5):
+    g = torch.Generator("cuda").manual_seed(seed)
+    return (scale * torch.randn(n, H, D, device="cuda", generator=g)).to(kind)
+
+
+# ---- append -----------------------------------------------------------------------------
+
+def append_reference(qkv, qw, kw, freq, pos, axis):
+    """q, gate [n, 16, 256], k, v [n, 4, 256] in 64 bits; pos [axes, n], axis [32]."""
+    x = qkv[:, :10240].double()
+    n = x.shape[0]
+    ang = torch.stack([pos[a].double() * freq[i].double() for i, a in enumerate(axis)], 1)[:, None]
+    c, s = ang.cos(), ang.sin()
+
+    def head(y, w):
+        y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + EPS) * w.double()
+        lo, hi = y[..., :32].clone(), y[..., 32:64].clone()
+        y[..., :32], y[..., 32:64] = lo * c - hi * s, lo * s + hi * c
+        return y
+
+    full = x[:, :8192].view(n, H, 2, D)
+    kv = x[:, 8192:].view(n, 2, KV, D)
+    return head(full[:, :, 0].clone(), qw), full[:, :, 1], head(kv[:, 0].clone(), kw), kv[:, 1]
+
+
+def axes_of(sections, interleaved):
+    if interleaved and len(sections) == 3:
+        return [i % 3 if i % 3 and i < 3 * sections[i % 3] else 0 for i in range(32)]
+    return [a for a, n in enumerate(sections) for _ in range(n)]
+
+
+FREQ = (1e7 ** (-torch.arange(32, dtype=torch.float64) / 32)).float()
+
+
+def near(y, ref, kind, norm):
+    """f32: 2^-20 of the row's scale `norm` (a 256-term sum, rsqrt and the turn: some 16 roundings of 2^-24); f16: that and half a step."""
+    tol = 2.0 ** -20 * norm + (2.0 ** -11 * ref.abs() + 2.0 ** -24 if kind == torch.float16 else 0)
+    err = (y.double() - ref).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("sections,interleaved", [((32,), True), ((11, 11, 10), True), ((11, 11, 10), False), ((20, 12), False),
+                                                  ((32, 0, 0), True)])
+def test_append_matches_the_formulas(half, q8, sections, interleaved):
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    # tokens of three rows in mixed order, chunk borders and the far end of the table, one padding token
+    where = [(0, 0), (2, 255), (2, 256), (1, 511), (0, 1), (-1, 7), (2, 257), (1, 300), (0, 767)]
+    c = Cache([768, 512, 300], q8, 3)
+    n = len(where)
+    g = torch.Generator("cuda").manual_seed(11)
+    wide = torch.randn(n, 10400, device="cuda", generator=g) * 3
+    qkv = wide[:, 4:10300] if half else wide[:, 3:10300]  # strided rows, also off a 16-byte border
+    qw, kw = (1 + 0.2 * torch.randn(256, device="cuda", generator=g) for _ in range(2))
+    pos = torch.randint(0, 262144, (len(sections), n), generator=torch.Generator().manual_seed(4)).int().cuda()
+    pos[:, 0] = 262143
+    seq, at = ints(*[w[0] for w in where]), ints(*[w[1] for w in where])
+    before = c.raw.clone()
+    q0 = torch.full((n, H, D), 7.0, dtype=kind, device="cuda")
+    q, gate = ops.attn_append(qkv, qw, kw, FREQ.cuda(), pos, sections, seq, at, c.ptrs(), c.k_off, c.v_off, eps=EPS,
+                              interleaved=interleaved, dtype=kind, kv_q8=q8, q=q0, gate=q0.clone())
+    rq, rg, rk, rv = append_reference(qkv, qw, kw, FREQ.cuda(), pos, axes_of(sections, interleaved))
+    real = [t for t in range(n) if where[t][0] >= 0]
+    near(q[real], rq[real], kind, rq.abs().amax(-1, keepdim=True)[real])
+    assert torch.equal(gate[real], rg[real].to(kind))
+    assert bool((q[5] == 7).all()) and bool((gate[5] == 7).all())
+    touched = torch.zeros(c.raw.shape[:2] + (KV, CH), dtype=torch.bool)
+    rows = c.rows()
+    for t in real:
+        s, p = where[t]
+        chunk = int(c.ids[s, p // CH])
+        touched[chunk, 2:, :, p % CH] = True
+        k, v = rows[chunk, 0, :, p % CH], rows[chunk, 1, :, p % CH]
+        if q8:
+            for got, ref in ((k, rk[t]), (v, rv[t])):
+                blocks = ref.view(KV, 8, 32)
+                d = blocks.abs().amax(-1, keepdim=True) / 127
+                value = got[..., 2:].view(torch.int8).double() * got[..., :2].view(torch.float16).double()
+                # half a step of d, the stored d's own rounding on up to 127 steps, and the f32 work before it
+                assert bool(((value - blocks).abs() <= d * (0.5 + 127 * 2.0 ** -11 + 0.01)).all())
+        else:
+            near(k, rk[t], torch.float16, rk[t].abs().amax(-1, keepdim=True))
+            assert torch.equal(v, rv[t].half())
+    same = (c.raw.view(*c.raw.shape[:2], KV, CH, -1) == before.view(*c.raw.shape[:2], KV, CH, -1)).all(-1).cpu()
+    assert bool(same[~touched].all())
+
+
+@pytest.mark.gpu
+def test_append_agrees_with_the_single_token_preprocess():
+    """One axis and near positions (where the f32 angle is exact enough): the same cache rows, q and gate."""
+    from qwowl35_b200 import ops
+    lens = [5, 260]
+    g = torch.Generator("cuda").manual_seed(2)
+    qkv = torch.randn(2, 10240, device="cuda", generator=g)
+    w = 1 + 0.1 * torch.randn(2, 256, device="cuda", generator=g)
+    a, b = Cache(lens, False, 1), Cache(lens, False, 1)
+    pos = ints(4, 259)
+    f = FREQ.cuda()
+    q1, g1 = ops.attn_preprocess(qkv, w[0].contiguous(), w[1].contiguous(), f, pos, a.ptrs(), a.k_off, a.v_off)
+    q2, g2 = ops.attn_append(qkv, w[0].contiguous(), w[1].contiguous(), f, pos[None].contiguous(), (32,), ints(0, 1), pos, b.ptrs(),
+                             b.k_off, b.v_off)
+    # the f32 angle of position 259 is off by at most 259 * 2^-24 rad
+    assert float((q1 - q2).abs().max()) <= 2.0 ** -15 * float(q2.abs().max()) and torch.equal(g1, g2)
+    ka, kb = a.rows().float(), b.rows().float()
+    assert torch.equal(ka.isnan(), kb.isnan())
+    assert bool(((ka - kb).nan_to_num().abs() <= 2.0 ** -10 * kb.nan_to_num().abs() + 2.0 ** -13).all())
+
+
+# ---- run attention -----------------------------------------------------------------------
+
+RUNS = [
+    [(0, 1)],
+    [(4095, 1)],
+    [(0, 300)],
+    [(255, 2), (1024, 7), (3000, 33), (0, 0), (100, 32)],
+    [(0, 31), (0, 32), (0, 33), (127, 1), (128, 1), (129, 64)],
+    [(700, 161), (9000, 5)],
+]
+CUTS = [(0, 0), (1, 0), (200, 4), (128, 300), (2 ** 31 - 1, 2 ** 31 - 1)]
+
+
+def prefill_case(runs, half, q8, window, sink, gate=True, seed=0, splits=None):
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    lens = [c + r for c, r in runs]
+    cache = Cache(lens, q8, seed + 1).fill(lens, seed + 2)
+    n = sum(r for _, r in runs)
+    q, gt = some(n + 3, seed + 3, kind), some(n + 3, seed + 4, kind, 1.0)
+    off = [0]
+    for _, r in runs:
+        off.append(off[-1] + r)
+    out = torch.full((n + 3, H * D), 5.0, dtype=kind, device="cuda")
+    ops.gqa_prefill(q, gt if gate else None, ints(*off), ints(*lens), max(r for _, r in runs), max(lens), cache.ptrs(),
+                    cache.k_off, cache.v_off, window=window, sink=sink, out=out, kv_q8=q8)
+    assert bool((out[n:] == 5).all())  # rows behind the last run
+    rows = []
+    for i, (c, r) in enumerate(runs):
+        k, v = cache.sequence(i, lens[i])
+        picks = sorted({0, 1, 30, 31, 32, 63, 64, r // 2, r - 2, r - 1} & set(range(r)))
+        for t in picks:
+            x = off[i] + t
+            rows.append((x, *attend(q[x], gt[x] if gate else None, k, v, c + t + 1, window, sink), c + t + 1))
+    check_rows(out, rows, half, q8)
+    assert _lib.lib().qw35_cuda_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("runs", RUNS)
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q8", [False, True])
+def test_prefill_matches_the_formula(runs, half, q8):
+    prefill_case(runs, half, q8, 0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sink", CUTS)
+@pytest.mark.parametrize("half,q8", [(True, False), (False, True)])
+def test_prefill_window_and_sink(window, sink, half, q8):
+    prefill_case([(300, 70), (0, 600), (2000, 3)], half, q8, window, sink)
+
+
+@pytest.mark.gpu
+def test_prefill_without_gate():
+    prefill_case([(100, 40)], True, False, 0, 0, gate=False)
+
+
+@pytest.mark.gpu
+def test_prefill_long_context():
+    prefill_case([(40000, 64)], False, False, 0, 0, seed=9)
+    prefill_case([(70001, 1), (3, 2)], True, True, 0, 0, seed=10)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+def test_prefill_rows_before_the_context_attend_nothing(half):
+    """A run longer than its context length: its first rows see no position and come out zero."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    cache = Cache([40], False, 5).fill([40], 6)
+    q, gt = some(50, 1, kind), some(50, 2, kind)
+    out = ops.gqa_prefill(q, gt, ints(0, 50), ints(40), 50, 40, cache.ptrs(), cache.k_off, cache.v_off)
+    assert bool((out[:10] == 0).all())
+    k, v = cache.sequence(0, 40)
+    check_rows(out, [(r, *attend(q[r], gt[r], k, v, r - 9), r - 9) for r in range(10, 50, 3)], half, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("scale", [1e-3, 8.0])
+def test_prefill_flat_and_peaked_scores(half, scale):
+    """Scores near zero (every position counts alike) and scores of hundreds (one position counts)."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    cache = Cache([900], False, 5).fill([900], 6)
+    q, gt = some(70, 1, kind, scale), some(70, 2, kind)
+    out = ops.gqa_prefill(q, gt, ints(0, 70), ints(900), 70, 900, cache.ptrs(), cache.k_off, cache.v_off)
+    k, v = cache.sequence(0, 900)
+    check_rows(out, [(r, *attend(q[r], gt[r], k, v, 831 + r), 831 + r) for r in range(0, 70, 7)], half, False)
+
+
+# ---- shared prefixes -----------------------------------------------------------------------
+
+def shared_case(groups, half, q8, window=0, sink=0, gate=True, seed=0, max_own=None):
+    """groups: [(shared length, [own lengths])]; an own length may be negative (the sequence ends inside the prefix)."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    lens = [max(0, s + o) for s, own in groups for o in own]
+    pre = [s for s, own in groups for _ in own]
+    cache = Cache([max(n, s) for n, s in zip(lens, pre)], q8, seed + 1)
+    cache.fill([max(n, s) for n, s in zip(lens, pre)], seed + 2)
+    at, off = 0, [0]
+    rows = cache.rows()
+    for s, own in groups:  # the prefix's whole chunks are one, its last part a copy
+        for j in range(at + 1, at + len(own)):
+            cache.ids[j, :s // CH] = cache.ids[at, :s // CH]
+            if s % CH:
+                rows[int(cache.ids[j, s // CH])][:, :, :s % CH] = rows[int(cache.ids[at, s // CH])][:, :, :s % CH]
+        at += len(own)
+        off.append(at)
+    n = len(lens)
+    q, gt = some(n, seed + 3, kind), some(n, seed + 4, kind, 1.0)
+    own_most = max(1, max(a - b for a, b in zip(lens, pre))) if max_own is None else max_own
+    args = (q, gt if gate else None, ints(*lens), ints(*off), ints(*[s for s, _ in groups]), max(s for s, _ in groups), own_most,
+            cache.ptrs(), cache.k_off, cache.v_off)
+    out = ops.gqa_decode_shared(*args, window=window, sink=sink, kv_q8=q8)
+    ref = []
+    for i, length in enumerate(lens):
+        k, v = cache.sequence(i, length)
+        ref.append((i, *attend(q[i], gt[i] if gate else None, k, v, length, window, sink), length))
+    check_rows(out, ref, half, q8)
+    assert _lib.lib().qw35_cuda_device_error() == 0
+    return cache, args, out, ref
+
+
+GROUPS = [
+    [(700, [3, 40])],
+    [(256, [1] * 33)],
+    [(1, [0])],
+    [(0, [17, 300])],
+    [(513, [0, 1, 255, 256, 600]), (0, [5]), (4096, [9]), (129, list(range(1, 70)))],
+    [(1000, [-999, -1000, -500, -1, 20])],
+    [(20000, [30, 1])],
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", GROUPS)
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q8", [False, True])
+def test_shared_matches_the_formula(groups, half, q8):
+    shared_case(groups, half, q8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sink", CUTS)
+@pytest.mark.parametrize("half,q8", [(False, False), (True, True)])
+def test_shared_window_and_sink(window, sink, half, q8):
+    shared_case([(500, [1, 30, 190, 260]), (260, [3, -200])], half, q8, window, sink)
+
+
+@pytest.mark.gpu
+def test_shared_without_gate_and_with_generous_bounds():
+    shared_case([(300, [4, 5])], False, False, gate=False, max_own=512)
+
+
+@pytest.mark.gpu
+def test_shared_agrees_with_gqa_decode():
+    from qwowl35_b200 import ops
+    cache, args, out, ref = shared_case([(777, [12, 90, 1]), (2048, [400])], False, False, seed=20)
+    q, gate, seq_len = args[:3]
+    plain = ops.gqa_decode(q, gate, seq_len, int(seq_len.max()), args[7], cache.k_off, cache.v_off)
+    check_rows(plain, ref, False, False)
+    check_rows(out, ref, False, False)
+
+
+# ---- together, captured, on several streams ---------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8", [(False, False), (True, False), (False, True)])
+def test_append_prefill_fork_and_shared_decode_together(half, q8):
+    """Two prompts enter the cache and attend; three continuations of the first then decode over its prefix."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    runs = [(0, 300), (0, 45)]
+    cache = Cache([600, 300, 600, 600], q8, 31)
+    cache.ids[2, 0] = cache.ids[3, 0] = cache.ids[0, 0]  # the whole chunk of the prompt is shared
+    g = torch.Generator("cuda").manual_seed(8)
+    qw, kw = (1 + 0.2 * torch.randn(256, device="cuda", generator=g) for _ in range(2))
+    qkv = torch.randn(345, 10240, device="cuda", generator=g)
+    pos = torch.cat([torch.arange(300), torch.arange(45)]).int().cuda()
+    seq = torch.cat([torch.zeros(300), torch.ones(45)]).int().cuda()
+    table, f = cache.ptrs(), FREQ.cuda()
+    q, gate = ops.attn_append(qkv, qw, kw, f, pos[None].repeat(3, 1), (11, 11, 10), seq, pos, table, cache.k_off, cache.v_off,
+                              dtype=kind, kv_q8=q8)
+    out = ops.gqa_prefill(q, gate, ints(0, 300, 345), ints(300, 45), 300, 300, table, cache.k_off, cache.v_off, kv_q8=q8)
+    rows = []
+    for i, (_, r) in enumerate(runs):
+        k, v = cache.sequence(i, r)
+        rows += [(300 * i + t, *attend(q[300 * i + t], gate[300 * i + t], k, v, t + 1), t + 1) for t in (0, 1, 31, 32, 44, r - 1)]
+    check_rows(out, rows, half, q8)
+    # fork: sequences 2 and 3 continue sequence 0 with their own copy of its last chunk
+    raw = cache.raw
+    for j in (2, 3):
+        raw[int(cache.ids[j, 1])] = raw[int(cache.ids[0, 1])]
+    order = [0, 2, 3]
+    tables = table[order].contiguous()
+    step = torch.randn(3, 10240, device="cuda", generator=g)
+    at = ints(300, 300, 300)
+    q, gate = ops.attn_append(step, qw, kw, f, at[None].contiguous(), (32,), ints(0, 1, 2), at, tables, cache.k_off, cache.v_off,
+                              dtype=kind, kv_q8=q8)
+    out = ops.gqa_decode_shared(q, gate, at + 1, ints(0, 3), ints(300), 300, 1, tables, cache.k_off, cache.v_off, kv_q8=q8)
+    rows = []
+    for r, i in enumerate(order):
+        k, v = cache.sequence(i, 301)
+        rows.append((r, *attend(q[r], gate[r], k, v, 301), 301))
+    check_rows(out, rows, half, q8)
+
+
+@pytest.mark.gpu
+def test_captured_calls_replay_over_other_lengths():
+    """One graph of both attentions, captured with upper bounds, replayed after the lengths on the device changed."""
+    from qwowl35_b200 import ops
+    cache = Cache([1500] * 4, False, 2).fill([1500] * 4, 3)
+    cache.ids[3, :2] = cache.ids[2, :2]
+    table = cache.ptrs()
+    q, gt = some(40, 1, torch.float32), some(40, 2, torch.float32)
+    off, lens = ints(0, 10, 40), ints(700, 800)
+    soff, slen, shared = ints(0, 2), ints(600, 520), ints(512)
+    out1, out2 = torch.zeros(40, 4096, device="cuda"), torch.zeros(2, 4096, device="cuda")
+    ws1, ws2 = ops.gqa_prefill_workspace(40, 2, 40, 1500), ops.gqa_decode_shared_workspace(2, 1, 512, 900)
+
+    def both():
+        ops.gqa_prefill(q, gt, off, lens, 40, 1500, table, cache.k_off, cache.v_off, ws=ws1, out=out1)
+        ops.gqa_decode_shared(q[:2], gt[:2], slen, soff, shared, 512, 900, table[2:], cache.k_off, cache.v_off, ws=ws2, out=out2)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for cut, n0, n1, s0, s1, sh in ((10, 700, 800, 600, 520, 512), (37, 1500, 3, 1400, 1, 500), (1, 20, 1499, 0, 512, 0)):
+        off.copy_(ints(0, cut, 40))
+        lens.copy_(ints(n0, n1))
+        slen.copy_(ints(s0, s1))
+        shared.copy_(ints(sh))
+        graph.replay()
+        rows = []
+        for i, (a, b, n) in enumerate(((0, cut, n0), (cut, 40, n1))):
+            k, v = cache.sequence(i, n)
+            rows += [(r, *attend(q[r], gt[r], k, v, n - (b - r) + 1), n - (b - r) + 1) for r in range(a, b, 3)]
+        check_rows(out1, rows, False, False)
+        rows = []
+        for i, n in enumerate((s0, s1)):
+            k, v = cache.sequence(2 + i, n)
+            rows.append((i, *attend(q[i], gt[i], k, v, n), n))
+        check_rows(out2, rows, False, False)
+
+
+@pytest.mark.gpu
+def test_two_streams_with_their_own_workspaces():
+    from qwowl35_b200 import ops
+    cache = Cache([3000, 2500], False, 2).fill([3000, 2500], 3)
+    q, gt = some(128, 1, torch.float16), some(128, 2, torch.float16)
+    want = [ops.gqa_prefill(q[64 * i:64 * i + 64], gt[64 * i:64 * i + 64], ints(0, 64), ints(n), 64, n, cache.ptrs()[i:i + 1].contiguous(),
+                            cache.k_off, cache.v_off) for i, n in enumerate((3000, 2500))]
+    tables = [cache.ptrs()[i:i + 1].contiguous() for i in range(2)]
+    off, lens = ints(0, 64), [ints(3000), ints(2500)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, n in enumerate((3000, 2500)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.gqa_prefill(q[64 * i:64 * i + 64], gt[64 * i:64 * i + 64], off, lens[i], 64, n, tables[i],
+                                              cache.k_off, cache.v_off))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y in got[i]:
+            assert torch.equal(y, want[i])  # no atomics: the same bits every time
+
+
+# ---- refusals (no GPU work) -----------------------------------------------------------------
+
+def _append_args(**over):
+    a = dict(n=4, qkv=16, stride=10240, qw=16, kw=16, freq=16, pos=16, axes=3, sec=(11, 11, 10), inter=1, seq=16, at=16, n_seq=2,
+             table=16, chunks=4, k=0, v=1 << 19, kv=0, q=16, gate=16, dtype=0)
+    a.update(over)
+    sec = (C.c_int32 * len(a["sec"]))(*a["sec"]) if a["sec"] is not None else None
+    return (a["n"], a["qkv"], a["stride"], a["qw"], a["kw"], a["freq"], a["pos"], a["axes"], sec, a["inter"], a["seq"], a["at"],
+            a["n_seq"], a["table"], a["chunks"], a["k"], a["v"], a["kv"], a["q"], a["gate"], a["dtype"], 1e-6, None)
+
+
+@pytest.mark.parametrize("over,message", [
+    (dict(qkv=None), "invalid append"), (dict(table=None), "invalid append"), (dict(seq=None), "invalid append"),
+    (dict(sec=None), "invalid append"), (dict(stride=10239), "invalid append"), (dict(n_seq=0), "invalid append"),
+    (dict(chunks=0), "invalid append"), (dict(k=8), "invalid append"), (dict(kv=2), "invalid append"), (dict(dtype=2), "invalid append"),
+    (dict(q=20), "invalid append"), (dict(axes=0), "rotary sections"), (dict(axes=4, sec=(8, 8, 8, 8)), "rotary sections"),
+    (dict(sec=(11, 11, 11)), "rotary sections"), (dict(sec=(33, -1, 0)), "rotary sections"),
+    (dict(sec=(1 << 31 - 1, 1 << 31 - 1, 34)), "rotary sections"), (dict(axes=2, sec=(20, 12)), "rotary sections"),
+])
+def test_append_refuses(over, message):
+    with pytest.raises(_lib.Qw35Error, match=message):
+        _lib.call("qw35_cuda_attn_append", *_append_args(**over))
+
+
+def test_calls_without_rows_do_nothing():
+    _lib.call("qw35_cuda_attn_append", *_append_args(n=0))
+    _lib.call("qw35_cuda_gqa_prefill", *_prefill_args(n=0))
+    _lib.call("qw35_cuda_gqa_decode_shared", *_shared_args(n=0))
+
+
+def _prefill_args(**over):
+    a = dict(n=4, q=16, gate=None, dtype=0, runs=1, off=16, len=16, max_run=4, max_len=100, table=16, chunks=1, k=0, v=1 << 19, kv=0,
+             window=0, sink=0, out=16, ws=16, bytes=1 << 40)
+    a.update(over)
+    return tuple(a.values()) + (None,)
+
+
+def _shared_args(**over):
+    a = dict(n=4, q=16, gate=None, dtype=0, len=16, groups=1, off=16, shared=16, max_shared=100, max_own=100, table=16, chunks=1,
+             k=0, v=1 << 19, kv=0, window=0, sink=0, out=16, ws=16, bytes=1 << 40)
+    a.update(over)
+    return tuple(a.values()) + (None,)
+
+
+@pytest.mark.parametrize("over", [dict(q=None), dict(q=8), dict(gate=8), dict(out=None), dict(off=None), dict(len=None), dict(dtype=2),
+                                  dict(table=None), dict(chunks=0), dict(max_len=257), dict(k=8), dict(v=8), dict(kv=2), dict(ws=None),
+                                  dict(n=1 << 25)])
+def test_prefill_refuses(over):
+    with pytest.raises(_lib.Qw35Error, match="invalid prefill"):
+        _lib.call("qw35_cuda_gqa_prefill", *_prefill_args(**over))
+
+
+@pytest.mark.parametrize("over", [dict(max_run=0), dict(max_run=5), dict(max_len=0)])
+def test_prefill_refuses_bounds(over):
+    with pytest.raises(_lib.Qw35Error, match="invalid prefill"):
+        _lib.call("qw35_cuda_gqa_prefill", *_prefill_args(**over))
+
+
+@pytest.mark.parametrize("over", [dict(q=None), dict(q=8), dict(gate=8), dict(out=None), dict(off=None), dict(len=None), dict(dtype=2),
+                                  dict(shared=None), dict(table=None), dict(chunks=0), dict(max_own=257), dict(max_shared=257), dict(k=8), dict(kv=2),
+                                  dict(max_shared=0, max_own=0), dict(n=65536), dict(max_shared=1 << 30, max_own=1 << 30)])
+def test_shared_refuses(over):
+    with pytest.raises(_lib.Qw35Error, match="invalid shared-prefix"):
+        _lib.call("qw35_cuda_gqa_decode_shared", *_shared_args(**over))
+
+
+def test_small_workspaces_are_refused():
+    need = _lib.lib().qw35_cuda_gqa_prefill_workspace_bytes(4, 1, 4, 100)
+    assert need > 0
+    with pytest.raises(_lib.Qw35Error, match="workspace too small"):
+        _lib.call("qw35_cuda_gqa_prefill", *_prefill_args(bytes=need - 1))
+    need = _lib.lib().qw35_cuda_gqa_decode_shared_workspace_bytes(4, 1, 100, 100)
+    assert need > 0
+    with pytest.raises(_lib.Qw35Error, match="workspace too small"):
+        _lib.call("qw35_cuda_gqa_decode_shared", *_shared_args(bytes=need - 1))
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_tensors_of_another_kind():
+    from qwowl35_b200 import ops
+    cache = Cache([40], False, 5).fill([40], 6)
+    q = some(4, 1, torch.float32)
+    good = (q, q, ints(0, 4), ints(40), 4, 40, cache.ptrs(), cache.k_off, cache.v_off)
+    ops.gqa_prefill(*good)
+    for at, bad in ((0, q.double()), (1, q.half()), (2, ints(0, 4).long()), (2, ints(0, 4, 4)), (6, cache.ptrs().float())):
+        with pytest.raises(TypeError):
+            ops.gqa_prefill(*good[:at], bad, *good[at + 1:])
+    with pytest.raises(ValueError):
+        ops.gqa_prefill(*good[:2], ints(0, 2, 4), ints(40, 40), *good[4:])
