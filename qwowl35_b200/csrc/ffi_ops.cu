@@ -56,7 +56,9 @@ int qw35_cuda_set_device(int device, char *err, uintptr_t err_len) {
     return cuda_ok(cudaSetDevice(device), "cudaSetDevice", err, err_len);
 }
 
-uint32_t qw35_cuda_device_error(void) { return qw35::device_error_read_and_clear(); }
+uint32_t qw35_cuda_device_error(void) {
+    return qw35::device_error_read_and_clear() | qw35::attn_tile_error_read_and_clear();
+}
 
 const char *qw35_cuda_build_info(void) { return "qw35cuda sm_100a (" __DATE__ ")"; }
 
@@ -331,7 +333,7 @@ int qw35_cuda_attn_append(uint32_t n_tok, const float *qkv, uint32_t qkv_stride,
     if (n_tok == 0) return 1;
     if (!qkv || !q_norm_w || !k_norm_w || !rope_freq || !rope_pos || !sections || !tok_seq || !tok_pos || !chunk_ptrs ||
         !q_out || !gate_out || qkv_stride < 10240 || n_seq == 0 || n_seq > (1u << 30) || max_chunks == 0 ||
-        max_chunks > (1u << 22) || n_tok > (1u << 30) || (k_off % 16) || (v_off % 16) || kv_type > 1 || dtype > 1 ||
+        max_chunks > (1u << 21) || n_tok > (1u << 30) || (k_off % 16) || (v_off % 16) || kv_type > 1 || dtype > 1 ||
         !aligned16(q_out) || !aligned16(gate_out)) {
         set_err(err, err_len, "invalid append arguments%s", "");
         return 0;
@@ -356,22 +358,22 @@ static bool tile_args(qw35::AttnTileArgs &a, uint32_t n_row, const void *q, cons
                       uint32_t n_run, const int32_t *off, const int32_t *len, uint64_t max_pos,
                       const uint64_t *chunk_ptrs, uint32_t max_chunks, uint64_t k_off, uint64_t v_off, uint32_t kv_type,
                       int32_t window, int32_t sink, void *out, void *ws, uint64_t ws_bytes) {
-    if (!q || !off || !len || !chunk_ptrs || !out || !ws || n_run == 0 || max_chunks == 0 || max_chunks > (1u << 22) ||
+    if (!q || !off || !len || !chunk_ptrs || !out || !ws || n_run == 0 || max_chunks == 0 || max_chunks > (1u << 21) ||
         (uint64_t)max_chunks * QW35_KV_CHUNK < max_pos || (k_off % 16) || (v_off % 16) || kv_type > 1 || dtype > 1 ||
         !aligned16(q) || !aligned16(gate) || !aligned16(out) || !aligned16(ws))
         return false;
     a.n_row = (int)n_row; a.n_run = (int)n_run; a.q = q; a.gate = gate; a.out = out; a.half = (int)dtype;
     a.off = off; a.len = len; a.chunk_ptrs = chunk_ptrs; a.max_chunks = (int)max_chunks;
     a.k_off = (long long)k_off; a.v_off = (long long)v_off; a.kv_q8 = (int)kv_type;
-    a.window = window < 0 ? 0 : (window > (1 << 30) ? 1 << 30 : window);
-    a.sink = sink < 0 ? 0 : (sink > (1 << 30) ? 1 << 30 : sink);
+    a.window = window < 0 ? 0 : (window > (1 << 29) ? 1 << 29 : window);  // (no length is above 2^29)
+    a.sink = sink < 0 ? 0 : (sink > (1 << 29) ? 1 << 29 : sink);
     a.ws = ws; a.ws_bytes = ws_bytes;
     return true;
 }
 
 // Limits of the size queries too: rows and runs within a grid, lengths within the table's.
 static bool tile_sizes_ok(uint32_t n_row, uint32_t n_run, uint64_t len) {
-    return n_row <= (1u << 24) && n_run <= 65535 && len <= (1u << 30);
+    return n_row <= (1u << 24) && n_run <= 65535 && len <= (1u << 29);
 }
 
 uint64_t qw35_cuda_gqa_prefill_workspace_bytes(uint32_t n_row, uint32_t n_run, uint32_t max_run, uint32_t max_len) {
