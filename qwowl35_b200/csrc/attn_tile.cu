@@ -5,25 +5,33 @@
 // p_j = exp(q . k_j / 16 - m) over what attended_range(L) keeps, then
 // o *= sigmoid(gate).
 //
-// One CTA takes a tile of up to 32 tokens (or sequences) x the 4 query heads of
-// one kv head = 128 rows, and walks 128-position tiles of K and V:
-//   S = Q K^T   128 x 128 x 256   tcgen05, A and B from shared memory
-//   P = exp2(S c - m c + 7)       8 warps, two per 32 rows, S and P in TMEM
-//   O += P V    128 x 256 x 128   tcgen05, A from TMEM, B from shared memory
+// A CTA takes a tile of up to 32 tokens (or sequences) x the 4 query heads of
+// one kv head = 128 rows, and walks position tiles of K and V:
+//   S = Q K^T   tcgen05, A and B from shared memory
+//   P = exp2(S c - m c + 7)   8 warps, two per 32 rows, S and P in TMEM
+//   O += P V    tcgen05, A from TMEM, B from shared memory
 // so that K and V are read once for all 128 rows.  TMEM holds O (256 columns)
-// and two S buffers (128 each): the score product of tile j + 1 runs while the
-// softmax warps work on tile j; P takes the place of its own S.  Chunks lie at
-// arbitrary addresses, which a tensor map cannot span, so four producer warps
-// copy K and V with cp.async (or turn q8_0 blocks into f16) into a ring of
-// 32 KB stages in the 128-byte swizzled layout.
+// and two S buffers: the score product of tile j + 1 runs while the softmax
+// warps work on tile j; P takes the place of its own S.  Chunks lie at arbitrary
+// addresses, which a tensor map cannot span, so producer warps copy K and V with
+// cp.async (or turn q8_0 blocks into f16) into a ring of stages in the 128-byte
+// swizzled layout, a stage a K or a V tile.
+//
+// What the ring holds decides the speed: a V tile waits in it for its softmax,
+// and the rest has to cover the latency of L2 or HBM.  Hence
+//   single CTAs   64 positions a tile; 5 stages of 32 KB beside Q (64 KB);
+//   CTA pairs     (runs of more than 32 tokens) 256 rows share one K/V tile, each
+//                 CTA holding half of it (cta_group::2): half the L2 reads and
+//                 twice the tiles in the ring.  128 positions a tile in f16.
+// f32 calls (HL) carry q and p as f16 hi + lo pairs, two products each, ~22
+// bits; Q's lo half sits in TMEM, where 64-position S buffers leave 128 columns,
+// so that the ring keeps its size.  q8_0 values d * code (18 bits) then enter as
+// hi + lo stages as well.  f16 calls round p to f16 once, and q8_0 values once,
+// the rounding their type implies.
 //
 // The running maximum is lazy: O is rescaled only when a row's maximum grows by
 // more than 2^8 over the one in use, so P reaches at most 2^15 (its 2^7 offset
 // keeps small probabilities out of f16's denormals).  Sums and O are f32.
-//
-// f32 calls (HL) carry q and p as f16 hi + lo pairs, two products each, ~22
-// bits; q8_0 values d * code (18 bits) then enter as hi + lo as well.  f16 calls
-// round p to f16 once, and q8_0 values once, the rounding their type implies.
 //
 // Work is split along the positions where there are few row tiles; the parts'
 // (m, l, O) go through the workspace and attn_join_kernel merges them.
@@ -37,34 +45,47 @@ namespace qw35 {
 
 namespace {
 
-constexpr int TM_ROWS = 128;             // rows of a tile: 32 tokens x 4 heads
-constexpr int TM_TOK = TM_ROWS / AGRP;   // tokens (sequences) of a tile
-constexpr int TK = 128;                  // positions of a K/V tile; divides a chunk
-constexpr int SOFT_WARPS = 8, LOAD_WARPS = 4;
-constexpr int TILE_THREADS = (SOFT_WARPS + LOAD_WARPS + 1) * 32;
-constexpr uint32_t STAGE = 32768;        // 128 positions x 128 dims of K, or 64 x 256 of V
+constexpr int TM_ROWS = 128;             // rows of a CTA: 32 tokens x 4 heads
+constexpr int TM_TOK = TM_ROWS / AGRP;   // tokens (sequences) of a CTA
+constexpr int SOFT_WARPS = 8;
 constexpr uint32_t QBYTES = TM_ROWS * AHD * 2;
 constexpr int kPlanSMs = 148;
+constexpr int kPlanTile = 128;           // positions by which work is divided: a whole number of any variant's tiles
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kShift = 7.0f, kSlack = 8.0f;  // log2: offset of P, growth of the maximum before O is rescaled
 
-template <bool HL>
+template <bool HL, bool Q8, bool PAIR>
 struct TileGeo {
-    static constexpr int NST = HL ? 3 : 5;  // stages: what 227 KB hold beside Q (hi and lo)
-    static constexpr int LAG = HL ? 1 : 2;  // copies of a producer thread in flight before it signals a stage
-    static constexpr uint32_t QB = HL ? 2 * QBYTES : QBYTES;
-    static constexpr uint32_t SMEM = QB + NST * STAGE;
+    static constexpr int CTAS = PAIR ? 2 : 1;
+    static constexpr int TK = PAIR && !HL ? 128 : 64;    // positions of a tile; divides a chunk
+    static constexpr int KR = TK / CTAS;                 // positions of K a CTA holds
+    static constexpr int VP = 32 / CTAS;                 // 16-byte pieces of a V row a CTA holds
+    static constexpr uint32_t STAGE = (uint32_t)TK * AHD * 2 / CTAS;
+    static constexpr int NST = 5 * 32768 / (int)STAGE;   // what 227 KB hold beside Q
+    // f16 planes: four warps issue the copies; q8_0: six convert, as many as fit 16 warps of 128 registers
+    static constexpr int LOADERS = Q8 ? 6 : 4;
+    static constexpr int THREADS = (SOFT_WARPS + LOADERS + 2) * 32;
+    [[maybe_unused]] static constexpr int WSTEPS = (int)STAGE / 512, STEPS = (WSTEPS + LOADERS - 1) / LOADERS;  // q8_0: a warp's passes over a stage
+    static constexpr int PARTS = HL && Q8 ? 2 : 1;       // stages of a tile: values, or their hi and lo halves
+    static constexpr uint32_t RING = NST * STAGE, SMEM = QBYTES + RING;
+    static constexpr uint32_t S0 = 256;       // TMEM columns
+    // f32: Q's lo half passes through the last 64 KB of the ring on its way to TMEM
+    static constexpr int FREE_AT_START = HL ? (int)((RING - QBYTES) / STAGE) : NST;
 };
 
 struct TilePlan {
+    int pair;       // row tiles of two CTAs
     int tiles;      // row tiles (upper bound)
     int ns;         // position splits of a row tile
     int own_tiles;  // shared prefixes: sequences with a tail of their own, else 0
     int ns_own;     // position splits of a tail
 };
 
+constexpr uint32_t kQlo = 384;  // TMEM columns of the lo half of Q
+constexpr int kMaxStages = 10;
 struct __align__(16) TileShared {
-    uint64_t full[5], empty[5], s_full[2], p_full[2], pv_done, q_full, o_full;
+    uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages];
+    uint64_t s_full[2], p_full[2], pv_done, q_full, q_moved, o_full;
     uint32_t tmem;
     int abort;
     int row0, nrow, kvh, table, part;  // this CTA's rows, kv head, chunk-table row, part number
@@ -74,9 +95,101 @@ struct __align__(16) TileShared {
     float ex[2][2][TM_ROWS];           // row maxima (then sums) exchanged between the two column halves
 };
 
+// ---- two CTAs ---------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cta_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// arrive on the leader's (rank 0's) copy of a barrier; MEM: this thread's (and its warp's) writes to memory go before it,
+// else only what a tcgen05 fence orders
+template <bool MEM>
+__device__ __forceinline__ void arrive_leader(uint64_t *bar) {
+    if constexpr (MEM)
+        asm volatile(
+            "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+            "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+            : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t *bar) {  // to both CTAs' copies
+    if constexpr (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                smem_u32(bar)),
+            "h"((unsigned short)3)
+            : "memory");
+    else
+        tc_commit(bar);
+}
+// D (+)= A B with A from shared memory / from TMEM, one CTA or the pair
+template <bool PAIR>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+            : "memory");
+    else
+        tc_mma_f16(d, a, b, idesc, acc);
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+            : "memory");
+    else
+        tc_mma_f16_ts(d, a, b, idesc, acc);
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_take(uint32_t *dst) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        tmem_alloc(dst, 512);
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_give(uint32_t tmem) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    else
+        tmem_dealloc(tmem, 512);
+}
+
+// Bounded wait (2 s, as mbar_wait) that sees the other CTA's writes too; after one has run out, none waits any more.
+__device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ void tw(uint64_t *bar, uint32_t parity, TileShared &s, unsigned code) {
-    if (*(volatile int *)&s.abort) return;
-    if (!mbar_wait(bar, parity, code)) *(volatile int *)&s.abort = 1;
+    if (*(volatile int *)&s.abort || try_wait_cluster(bar, parity)) return;
+    const unsigned long long t0 = globaltimer();
+    while (!try_wait_cluster(bar, parity)) {
+        if (globaltimer() - t0 > kTimeoutNs) {
+            atomicOr(&g_dev_error, code);
+            *(volatile int *)&s.abort = 1;
+            return;
+        }
+    }
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -90,10 +203,10 @@ __device__ __forceinline__ void cpa16(uint32_t dst, const void *src, bool valid)
 }
 
 // V stage as the B operand of O += P V: dims contiguous ("MN-major"), rows of 128 bytes (64 dims) per position,
-// 128-byte swizzle; 64-dim blocks 8 KB apart (LBO), 8-position groups 1 KB apart (SBO)
-__device__ __forceinline__ uint64_t desc_v(uint32_t saddr) {
-    uint64_t d = smem_desc_sw128(saddr);
-    return (d & ~((uint64_t)0x3FFFu << 16)) | ((uint64_t)(8192u >> 4) << 16);
+// 128-byte swizzle; 64-dim blocks `block` bytes apart (LBO), 8-position groups 1 KB apart (SBO)
+__device__ __forceinline__ uint64_t desc_v(uint32_t saddr, uint32_t block) {
+    const uint64_t d = smem_desc_sw128(saddr);
+    return (d & ~((uint64_t)0x3FFFu << 16)) | ((uint64_t)(block >> 4) << 16);
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -106,6 +219,28 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo = pack2(a - f.x, b - f.y);
 }
 
+// 8 consecutive values of a row, 16-byte aligned
+__device__ __forceinline__ void get8(const float *p, float *v) {
+    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void get8(const __half *p, float *v) {
+    const uint4 u = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        v[2 * i] = t.x;
+        v[2 * i + 1] = t.y;
+    }
+}
+__device__ __forceinline__ void put8(float *p, const float *v) {
+    *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void put8(__half *p, const float *v) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+}
 __device__ __forceinline__ int warp_min_i(int v) { return __reduce_min_sync(0xffffffffu, v); }
 __device__ __forceinline__ int warp_max_i(int v) { return __reduce_max_sync(0xffffffffu, v); }
 
@@ -121,12 +256,12 @@ __device__ __forceinline__ int run_of_row(const AttnTileArgs &p, int r) {
 }
 
 // Row tile `tile` -> its run and first row, by one converged warp; false behind the last tile.
-__device__ __forceinline__ bool find_tile(const AttnTileArgs &p, int tile, int &run, int &row0) {
+__device__ __forceinline__ bool find_tile(const AttnTileArgs &p, int tile, int toks, int &run, int &row0) {
     const int lane = threadIdx.x & 31;
     int before = 0;
     for (int u = 0; u < p.n_run; u += 32) {
         const int a = u + lane < p.n_run ? p.off[u + lane] : 0, b = u + lane < p.n_run ? p.off[u + lane + 1] : 0;
-        const int n = b > a ? (b - a + TM_TOK - 1) / TM_TOK : 0;
+        const int n = b > a ? (b - a + toks - 1) / toks : 0;
         int sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -137,7 +272,7 @@ __device__ __forceinline__ bool find_tile(const AttnTileArgs &p, int tile, int &
         if (hit) {
             const int w = __ffs(hit) - 1;
             run = u + w;
-            row0 = __shfl_sync(0xffffffffu, a + (tile - (before + sum - n)) * TM_TOK, w);
+            row0 = __shfl_sync(0xffffffffu, a + (tile - (before + sum - n)) * toks, w);
             return true;
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
@@ -145,53 +280,64 @@ __device__ __forceinline__ bool find_tile(const AttnTileArgs &p, int tile, int &
     return false;
 }
 
-// What this CTA does, by warp 0; begin = end = 0 and nrow = 0 when there is no such unit.
-__device__ __forceinline__ void find_work(const AttnTileArgs &p, const TilePlan &pl, TileShared &s) {
+// What this CTA does, by warp 0; false when there is no such unit (for both CTAs of a pair).
+template <int CTAS, int TK>
+__device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan &pl, TileShared &s, int rank) {
     const int lane = threadIdx.x & 31;
-    int id = blockIdx.x, run = -1, row0 = 0, nrow = 0, ns = pl.ns, split;
+    int id = blockIdx.x / CTAS, run = -1, row0 = 0, nrow = 0, ns = pl.ns, split, kvh;
     const int n_first = pl.tiles * AKV * pl.ns;
     const bool tail = id >= n_first;
     if (!tail) {
         split = id % ns;
-        s.kvh = (id / ns) % AKV;
+        kvh = (id / ns) % AKV;
         int tile = id / (AKV * ns);
         if (!p.shared_len) tile = pl.tiles - 1 - tile;  // the last tokens of a run have the most to do: first
-        if (find_tile(p, tile, run, row0)) nrow = min(TM_TOK, p.off[run + 1] - row0);
+        if (find_tile(p, tile, TM_TOK * CTAS, run, row0)) nrow = min(TM_TOK * CTAS, p.off[run + 1] - row0);
     } else {
         id -= n_first;
         ns = pl.ns_own;
         split = id % ns;
-        s.kvh = (id / ns) % AKV;
+        kvh = (id / ns) % AKV;
         row0 = id / (AKV * ns);
         run = run_of_row(p, row0);
         nrow = run >= 0 ? 1 : 0;
     }
     if (row0 < 0 || row0 + nrow > p.n_row) nrow = 0;
-    // lane = token of the tile
-    const bool real = lane < nrow;
-    int hi = 0, sk = 0, rs = 0, lo = 0;
-    if (real) {
-        const int r = row0 + lane;
-        int L = p.shared_len ? p.len[r] : p.len[run] - (p.off[run + 1] - p.off[run]) + (r - p.off[run]) + 1;
-        L = max(0, min(L, p.max_chunks * ACHUNK));
-        int total;
-        attended_range(L, p.window, p.sink, total, sk, rs);
-        hi = L;
-        if (p.shared_len) {
-            const int sh = max(0, p.shared_len[run]);
-            if (tail) lo = sh;
-            else hi = min(L, sh);
+    // lane = token of the CTA's tile; a pair walks the positions that either of its tiles needs
+    int lo = 0, hi_max = 0, rs_min = 0x7fffffff, sk_max = 0;
+    for (int e = 0; e < CTAS; ++e) {
+        const int tok = e * TM_TOK + lane;
+        const bool real = tok < nrow;
+        int hi = 0, sk = 0, rs = 0;
+        if (real) {
+            const int r = row0 + tok;
+            int L = p.shared_len ? p.len[r] : p.len[run] - (p.off[run + 1] - p.off[run]) + (r - p.off[run]) + 1;
+            L = max(0, min(L, p.max_chunks * ACHUNK));
+            int total;
+            attended_range(L, p.window, p.sink, total, sk, rs);
+            hi = L;
+            if (p.shared_len) {
+                const int sh = max(0, p.shared_len[run]);
+                if (tail) lo = sh;
+                else hi = min(L, sh);
+            }
+        }
+        hi_max = max(hi_max, warp_max_i(hi));
+        rs_min = min(rs_min, warp_min_i(real && hi > 0 ? rs : 0x7fffffff));
+        sk_max = max(sk_max, warp_max_i(sk));
+        if (e == rank) {
+            s.hi[lane] = hi;
+            s.sk[lane] = sk;
+            s.rs[lane] = rs;
+            const int hi_min = warp_min_i(real ? hi : 0x7fffffff), rs_max = warp_max_i(rs);
+            if (lane == 0) {
+                s.hi_min = hi_min;
+                s.rs_max = rs_max;
+            }
         }
     }
-    if (lane < TM_TOK) {
-        s.hi[lane] = hi;
-        s.sk[lane] = sk;
-        s.rs[lane] = rs;
-    }
     lo = warp_max_i(lo);
-    const int hi_max = warp_max_i(hi), hi_min = warp_min_i(real ? hi : 0x7fffffff);
-    const int rs_min = warp_min_i(real && hi > 0 ? rs : 0x7fffffff), rs_max = warp_max_i(rs);
-    const int sk_end = min(warp_max_i(sk), hi_max);
+    const int sk_end = min(sk_max, hi_max);
     const int end = (hi_max + TK - 1) / TK, a0 = lo / TK;
     const int a1 = sk_end > lo ? (sk_end + TK - 1) / TK : a0;
     int t2 = max(lo, min(rs_min, hi_max)) / TK, n1 = a1 - a0;
@@ -201,187 +347,253 @@ __device__ __forceinline__ void find_work(const AttnTileArgs &p, const TilePlan 
     }
     const int total = hi_max > lo ? n1 + max(0, end - t2) : 0;
     if (lane == 0) {
-        s.row0 = row0;
-        s.nrow = nrow;
+        s.row0 = row0 + rank * TM_TOK;
+        s.nrow = max(0, min(TM_TOK, nrow - rank * TM_TOK));
+        s.kvh = kvh;
         s.table = p.shared_len ? (tail ? row0 : (run >= 0 ? p.off[run] : 0)) : max(run, 0);
         s.part = tail ? pl.ns + split : split;
-        s.lo = lo; s.hi_max = hi_max; s.hi_min = hi_min; s.rs_max = rs_max;
+        s.lo = lo; s.hi_max = hi_max;
         s.a0 = a0; s.n1 = n1; s.t2 = t2;
         s.begin = (int)((long long)total * split / ns);
         s.end = (int)((long long)total * (split + 1) / ns);
     }
+    return nrow > 0;
 }
 
 __device__ __forceinline__ int tile_at(const TileShared &s, int i) { return i < s.n1 ? s.a0 + i : s.t2 + (i - s.n1); }
 
-// 8 values of a q8_0 row (block c / 4, quarter c % 4) as f16, rounded (lo null) or as exact hi + lo halves
-template <bool HL>
-__device__ __forceinline__ void q8_piece(const uint8_t *row, int c, uint4 &hi, uint4 &lo) {
-    const uint8_t *blk = row + 34 * (c >> 2);
-    const float d = __half2float(*reinterpret_cast<const __half *>(blk));
-    const unsigned short *qd = reinterpret_cast<const unsigned short *>(blk + 2 + 8 * (c & 3));
-    uint32_t h[4], l[4];
+// 8 codes of a q8_0 block (quarter j of the block at blk, 34 b bytes into its row) as they lie in memory: the
+// codes start 2 or 0 bytes past a 4-byte border by the block's parity, and only the words they touch are read
+struct Q8Raw {
+    uint32_t w0, w1, w2;
+    unsigned short d;
+};
+__device__ __forceinline__ Q8Raw q8_fetch(const uint8_t *blk, int j, bool odd) {
+    Q8Raw r;
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(blk + 2 + 8 * j - (odd ? 0 : 2));
+    r.d = *reinterpret_cast<const unsigned short *>(blk);
+    r.w0 = w[0];
+    r.w1 = w[1];
+    r.w2 = odd ? 0u : w[2];
+    return r;
+}
+// d * code in f16: h rounded, l the remainder, exact (18 bits of product, 11 in h)
+__device__ __forceinline__ void q8_halves(const Q8Raw &r, bool odd, uint4 &h, uint4 &l) {
+    const uint32_t sh = odd ? 0u : 16u;
+    const uint32_t x[2] = {__funnelshift_r(r.w0, r.w1, sh) ^ 0x80808080u, __funnelshift_r(r.w1, r.w2, sh) ^ 0x80808080u};
+    const __half2 d = __half2half2(__ushort_as_half(r.d)), bias = __half2half2(__ushort_as_half((unsigned short)0x6480));
+    uint32_t hw[4], lw[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t two = qd[i];
-        const float a = d * (float)(int8_t)(two & 0xffu), b = d * (float)(int8_t)(two >> 8);
-        if constexpr (HL) split2(a, b, h[i], l[i]);
-        else h[i] = pack2(a, b);
+    for (int i = 0; i < 4; ++i) {  // bytes of code + 128 in halves 1024 + byte; - 1152 is exact
+        const uint32_t v = __byte_perm(x[i >> 1], 0x64646464u, (i & 1) ? 0x4342u : 0x4140u);
+        const __half2 q = __hsub2(*reinterpret_cast<const __half2 *>(&v), bias);
+        const __half2 hi = __hmul2(q, d), lo = __hfma2(q, d, __hneg2(hi));
+        hw[i] = *reinterpret_cast<const uint32_t *>(&hi);
+        lw[i] = *reinterpret_cast<const uint32_t *>(&lo);
     }
-    hi = make_uint4(h[0], h[1], h[2], h[3]);
-    if constexpr (HL) lo = make_uint4(l[0], l[1], l[2], l[3]);
+    h = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+    l = make_uint4(lw[0], lw[1], lw[2], lw[3]);
 }
 
 __device__ __forceinline__ void sts16(uint32_t dst, const uint4 &v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+__device__ __forceinline__ void lds16(uint32_t src, uint32_t *v) {
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
+}
+
 // ---- producers ------------------------------------------------------------------
-template <bool HL, bool Q8>
+// Stages in the order in which the products consume them: K(0), then K(j + 1) before V(j).  A pair's CTA holds half
+// of each: K by positions, V by dims.  Rows outside [lo, hi) (and of a chunk that is missing) come in as zeros.
+struct TileRef {
+    uint64_t plane;    // this layer's K or V plane of the chunk; 0: missing
+    int pos0, row0;    // position and plane row of the stage's first row
+    bool v;
+};
+
+template <bool HL, bool Q8, bool PAIR>
 struct Loader {
-    using G = TileGeo<HL>;
+    using G = TileGeo<HL, Q8, PAIR>;
     const AttnTileArgs &p;
     TileShared &s;
     uint32_t ring;
-    int tid, issued = 0, told = 0;
+    int tid, rank, lo, hi, n, slot = 0;
+    uint32_t phase = 1;  // parity that the slot's last release has; the first round waits for none
 
-    __device__ __forceinline__ void signal() {  // the oldest unsignalled stage is written (by this thread)
-        fence_async_smem();
-        __syncwarp();
-        if ((tid & 31) == 0) mbar_arrive(&s.full[told % G::NST]);
-        ++told;
+    __device__ __forceinline__ TileRef ref(int i) const {  // 0: K(0); 2 j + 1: K(j + 1); 2 j + 2: V(j); the last: V(n - 1)
+        TileRef h;
+        h.v = i == 2 * n - 1 || (i > 0 && !(i & 1));
+        const int j = i == 2 * n - 1 ? n - 1 : (h.v ? i / 2 - 1 : (i + 1) / 2);
+        const int t = tile_at(s, s.begin + j);
+        const uint64_t base = p.chunk_ptrs[(size_t)s.table * p.max_chunks + t / (ACHUNK / G::TK)];
+        h.plane = base ? base + (h.v ? p.v_off : p.k_off) : 0;
+        h.pos0 = t * G::TK + (h.v ? 0 : rank * G::KR);
+        h.row0 = s.kvh * ACHUNK + h.pos0 % ACHUNK;
+        return h;
     }
-    __device__ __forceinline__ uint32_t acquire() {
-        const int slot = issued % G::NST;
-        if (issued >= G::NST) tw(&s.empty[slot], (uint32_t)(issued / G::NST - 1) & 1u, s, 1u);
-        ++issued;
-        return ring + slot * STAGE;
+    // next free stage
+    __device__ __forceinline__ int acquire(int stage) {
+        const int k = slot;
+        if (stage >= G::NST) tw(&s.empty[k], phase, s, 1u);
+        else if (stage >= G::FREE_AT_START) tw(&s.q_moved, 0, s, 512u);
+        if (++slot == G::NST) {
+            slot = 0;
+            phase ^= 1u;
+        }
+        return k;
     }
-    // half 0 / 1 of K (dims) or V (positions) of position tile t
+
+    // f16 planes: asynchronous copies of 16 bytes; the last to land signals the stage
     template <bool V>
-    __device__ __forceinline__ void half_tile(int t, int half) {
-        const uint64_t base = p.chunk_ptrs[(size_t)s.table * p.max_chunks + t / (ACHUNK / TK)];
-        const uint64_t plane = base + (V ? p.v_off : p.k_off);
-        // rows outside [lo, hi) (and of a chunk that is missing) come in as zeros
-        const int lo = s.lo, hi = base ? s.hi_max : 0;
-        const int pos0 = t * TK + (V ? half * 64 : 0);
-        const size_t row0 = (size_t)s.kvh * ACHUNK + pos0 % ACHUNK;
-        constexpr int PC = V ? 32 : 16;       // 16-byte pieces of f16 a row of the stage has
-        constexpr int RP = LOAD_WARPS * 32 / PC, N = (V ? 64 : 128) / RP;
+    __device__ __forceinline__ void copy(const TileRef &h, int stage) {
+        constexpr int PC = V ? G::VP : 32;  // pieces of a row of the stage
+        constexpr int ROWS = V ? G::TK : G::KR, RP = G::LOADERS * 32 / PC, N = ROWS / RP;
         const int c = tid % PC, r0 = tid / PC;
-        const uint32_t blk = (uint32_t)(c >> 3) * (V ? 8192u : 16384u);
-        if constexpr (Q8) {
-            const uint32_t d0 = acquire(), d1 = HL ? acquire() : 0u;
-#pragma unroll 4
-            for (int i = 0; i < N; ++i) {
-                const int r = r0 + i * RP, pos = pos0 + r;
-                uint4 vh = make_uint4(0, 0, 0, 0), vl = vh;
-                if (pos >= lo && pos < hi)
-                    q8_piece<HL>(reinterpret_cast<const uint8_t *>(plane) + (row0 + r) * kKvQ8Row, c + (V ? 0 : half * 16), vh, vl);
-                const uint32_t at = blk + sw128_off(r, c & 7);
-                sts16(d0 + at, vh);
-                if constexpr (HL) sts16(d1 + at, vl);
-            }
-            signal();
-            if constexpr (HL) signal();
-        } else {
-            const uint32_t d0 = acquire();
-            const uint8_t *src = reinterpret_cast<const uint8_t *>(plane) + (row0 + r0) * (AHD * 2) + (V ? 0 : half * 256) + c * 16;
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(h.plane) + (size_t)(h.row0 + r0) * (AHD * 2) + ((V ? rank * G::VP : 0) + c) * 16;
+        const int k = acquire(stage);
+        const uint32_t dst = ring + k * G::STAGE + (uint32_t)(c >> 3) * (ROWS * 128u);
+        const int a = lo - h.pos0, b = (h.plane ? hi : 0) - h.pos0;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int r = r0 + i * RP, pos = pos0 + r;
-                const bool ok = pos >= lo && pos < hi;
-                cpa16(d0 + blk + sw128_off(r, c & 7), ok ? static_cast<const void *>(src + (size_t)i * RP * AHD * 2) : p.q, ok);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (issued > G::LAG) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(G::LAG) : "memory");
-                signal();
-            }
+        for (int i = 0; i < N; ++i) {
+            const int r = r0 + i * RP;
+            const bool ok = r >= a && r < b;
+            cpa16(dst + sw128_off(r, c & 7), ok ? static_cast<const void *>(src + (size_t)i * RP * AHD * 2) : p.q, ok);
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.full[k])) : "memory");
+    }
+
+    // q8_0 planes: a warp takes 32 pieces (a row of K, one or two of V) per step; the words of a stage are fetched
+    // while the one before it is converted
+    __device__ __forceinline__ int piece(bool v) const { return v ? rank * G::VP + (tid & 31) % G::VP : tid & 31; }
+    __device__ __forceinline__ int step_row(bool v, int step) const { return v ? step * G::CTAS + (tid & 31) / G::VP : step; }
+    __device__ __forceinline__ void fetch(const TileRef &h, Q8Raw *raw) const {
+        const int c = piece(h.v);
+#pragma unroll
+        for (int i = 0; i < G::STEPS; ++i) {
+            const int step = (tid >> 5) + i * G::LOADERS, r = step_row(h.v, step), pos = h.pos0 + r;
+            if (step < G::WSTEPS && pos >= lo && pos < hi && h.plane)
+                raw[i] = q8_fetch(reinterpret_cast<const uint8_t *>(h.plane) + (size_t)(h.row0 + r) * kKvQ8Row + 34 * (c >> 2), c & 3, (c >> 2) & 1);
+            else
+                raw[i] = Q8Raw{0u, 0u, 0u, 0};
         }
     }
-    template <bool V>
-    __device__ __forceinline__ void tile(int t) {
-        half_tile<V>(t, 0);
-        half_tile<V>(t, 1);
+    __device__ __forceinline__ void convert(const TileRef &h, const Q8Raw *raw, int stage) {
+        const int c = piece(h.v), cs = h.v ? c - rank * G::VP : c;
+        const uint32_t blk = (uint32_t)(cs >> 3) * (h.v ? G::TK * 128u : G::KR * 128u);
+        const int k0 = acquire(stage * G::PARTS), k1 = HL ? acquire(stage * G::PARTS + 1) : 0;
+        const uint32_t d0 = ring + k0 * G::STAGE + blk, d1 = ring + k1 * G::STAGE + blk;
+#pragma unroll
+        for (int i = 0; i < G::STEPS; ++i) {
+            const int step = (tid >> 5) + i * G::LOADERS, r = step_row(h.v, step);
+            if (step < G::WSTEPS) {
+                uint4 vh, vl;
+                q8_halves(raw[i], (c >> 2) & 1, vh, vl);
+                sts16(d0 + sw128_off(r, cs & 7), vh);
+                if constexpr (HL) sts16(d1 + sw128_off(r, cs & 7), vl);
+            }
+        }
+        mbar_arrive(&s.full[k0]);
+        if constexpr (HL) mbar_arrive(&s.full[k1]);
     }
-    // K(0), then K(j + 1) before V(j): the order in which the products consume them
+
     __device__ __forceinline__ void run() {
-        const int n = s.end - s.begin;
-        if (n > 0) tile<false>(tile_at(s, s.begin));
-        for (int j = 0; j < n; ++j) {
-            if (j + 1 < n) tile<false>(tile_at(s, s.begin + j + 1));
-            tile<true>(tile_at(s, s.begin + j));
+        if (n <= 0) return;
+        if constexpr (Q8) {
+            Q8Raw a[G::STEPS], b[G::STEPS];
+            TileRef ha = ref(0), hb;
+            fetch(ha, a);
+            for (int i = 0; i < 2 * n; i += 2) {
+                hb = ref(i + 1);
+                fetch(hb, b);
+                convert(ha, a, i);
+                if (i + 2 < 2 * n) {
+                    ha = ref(i + 2);
+                    fetch(ha, a);
+                }
+                convert(hb, b, i + 1);
+            }
+        } else {
+            for (int i = 0; i < 2 * n; ++i) {
+                const TileRef h = ref(i);
+                if (h.v) copy<true>(h, i);
+                else copy<false>(h, i);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        while (told < issued) signal();
     }
 };
 
-// ---- products (one thread) --------------------------------------------------------
-template <bool HL, bool Q8>
+// ---- products (one warp; of a pair, the leader's) ------------------------------------
+template <bool HL, bool Q8, bool PAIR>
 struct Products {
-    using G = TileGeo<HL>;
+    using G = TileGeo<HL, Q8, PAIR>;
     TileShared &s;
     uint32_t q, ring, tmem;
-    int used = 0;
+    int slot = 0;
+    uint32_t phase = 0;
 
-    static constexpr int PARTS = HL && Q8 ? 2 : 1;  // stages of a K or V half: values, or hi then lo
-    __device__ __forceinline__ uint32_t next() {
-        const int slot = used % G::NST;
-        tw(&s.full[slot], (uint32_t)(used / G::NST) & 1u, s, 2u);
-        return ring + slot * STAGE;
+    // stage `slot + ahead` is there (in both CTAs)
+    __device__ __forceinline__ uint32_t stage(int ahead) {
+        const int k = slot + ahead >= G::NST ? slot + ahead - G::NST : slot + ahead;
+        tw(&s.ready[k], phase ^ (slot + ahead >= G::NST ? 1u : 0u), s, 2u);
+        return ring + k * G::STAGE;
     }
-    __device__ __forceinline__ void done() {
-        tc_commit(&s.empty[used % G::NST]);
-        ++used;
+    __device__ __forceinline__ void release() {
+        if (elect_one()) commit<PAIR>(&s.empty[slot]);
+        if (++slot == G::NST) {
+            slot = 0;
+            phase ^= 1u;
+        }
     }
+    // S = Q K^T; f32: the small products first, so that the accumulator is rounded at full size only 16 times
     __device__ __forceinline__ void scores(int j) {
-        const uint32_t d = tmem + 256 + (j & 1) * 128;
-        constexpr uint32_t idesc = idesc_f16_f32(TM_ROWS, TK);
+        const uint32_t d = tmem + G::S0 + (j & 1) * G::TK;
+        constexpr uint32_t idesc = idesc_f16_f32(TM_ROWS * G::CTAS, G::TK);
+        const uint32_t k0 = stage(0), k1 = G::PARTS > 1 ? stage(1) : k0;
+        const uint64_t kd0 = smem_desc_sw128(k0), kd1 = smem_desc_sw128(k1), qd = smem_desc_sw128(q);
+        // descriptors hold addresses in units of 16 bytes: 32 bytes a step of 16 dims, a block every 64 dims
+        auto kstep = [](int i) { return (uint64_t)((i >> 2) * (G::KR * 8) + (i & 3) * 2); };
+        auto qstep = [](int i) { return (uint64_t)((i >> 2) * 1024 + (i & 3) * 2); };
+        if (elect_one()) {
+            if constexpr (HL) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+                for (int i = 0; i < 16; ++i) mma_ts<PAIR>(d, tmem + kQlo + i * 8, kd0 + kstep(i), idesc, i > 0);
+                if constexpr (Q8) {
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-                const uint32_t k = next();
-                tc_fence_after();
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        const uint32_t a = q + (half * 2 + b) * 16384 + ks * 32;
-                        const uint64_t bd = smem_desc_sw128(k + b * 16384 + ks * 32);
-                        tc_mma_f16(d, smem_desc_sw128(a), bd, idesc, !(half == 0 && part == 0 && b == 0 && ks == 0));
-                        if (HL && part == 0) tc_mma_f16(d, smem_desc_sw128(a + QBYTES), bd, idesc, 1);
-                    }
-                done();
-            }
-        tc_commit(&s.s_full[j & 1]);
-    }
-    __device__ __forceinline__ void values(int j) {
-        const uint32_t pa = tmem + 256 + (j & 1) * 128;
-        constexpr uint32_t idesc = idesc_f16_f32(TM_ROWS, AHD) | (1u << 16);  // B MN-major
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-                const uint32_t v = next();
-                tc_fence_after();
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) {
-                    const uint64_t bd = desc_v(v + ks * 2048);
-                    const uint32_t a = pa + half * 32 + ks * 8;
-                    tc_mma_f16_ts(tmem, a, bd, idesc, !(j == 0 && half == 0 && part == 0 && ks == 0));
-                    if (HL && part == 0) tc_mma_f16_ts(tmem, a + 64, bd, idesc, 1);
+                    for (int i = 0; i < 16; ++i) mma_ss<PAIR>(d, qd + qstep(i), kd1 + kstep(i), idesc, 1);
                 }
-                done();
             }
-        tc_commit(&s.pv_done);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mma_ss<PAIR>(d, qd + qstep(i), kd0 + kstep(i), idesc, HL || i > 0);
+            commit<PAIR>(&s.s_full[j & 1]);
+        }
+        __syncwarp();
+        for (int e = 0; e < G::PARTS; ++e) release();
+    }
+    // O += P V
+    __device__ __forceinline__ void values(int j) {
+        const uint32_t pa = tmem + G::S0 + (j & 1) * G::TK;
+        constexpr uint32_t idesc = idesc_f16_f32(TM_ROWS * G::CTAS, AHD) | (1u << 16);  // B MN-major
+        const uint32_t v0 = stage(0), v1 = G::PARTS > 1 ? stage(1) : v0;
+        const uint64_t vd0 = desc_v(v0, G::TK * 128u), vd1 = desc_v(v1, G::TK * 128u);
+        if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < G::TK / 16; ++i) {  // 16 positions: 2048 bytes on
+                if constexpr (HL) mma_ts<PAIR>(tmem, pa + G::TK / 2 + i * 8, vd0 + i * 128, idesc, j > 0 || i > 0);
+                if constexpr (HL && Q8) mma_ts<PAIR>(tmem, pa + i * 8, vd1 + i * 128, idesc, 1);
+                mma_ts<PAIR>(tmem, pa + i * 8, vd0 + i * 128, idesc, HL || j > 0 || i > 0);
+            }
+            commit<PAIR>(&s.pv_done);
+        }
+        __syncwarp();
+        for (int e = 0; e < G::PARTS; ++e) release();
     }
     __device__ __forceinline__ void run() {
         const int n = s.end - s.begin;
         if (n <= 0) return;
         tw(&s.q_full, 0, s, 4u);
+        tc_fence_after();
         scores(0);
         for (int j = 0; j < n; ++j) {
             if (j + 1 < n) scores(j + 1);  // into the buffer whose P the product before last has consumed, in order
@@ -389,125 +601,202 @@ struct Products {
             tc_fence_after();
             values(j);
         }
-        tc_commit(&s.o_full);
+        if (elect_one()) commit<PAIR>(&s.o_full);
+        __syncwarp();
         // after a timeout nobody else may be waiting: let the products end before TMEM is freed
         if (*(volatile int *)&s.abort) mbar_wait(&s.o_full, 0, 16u);
     }
 };
 
+// A thread of each CTA makes the producers' ordinary writes, seen through `full`, visible to the products and tells
+// their warp: the fence costs the products' warp 0.1 us a stage otherwise.
+template <bool HL, bool Q8, bool PAIR>
+__device__ __forceinline__ void relay(TileShared &s, int rank) {
+    using G = TileGeo<HL, Q8, PAIR>;
+    const int n = 2 * G::PARTS * (s.end - s.begin);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < n; ++i) {
+        tw(&s.full[slot], phase, s, 2u);
+        fence_async_smem();
+        if (PAIR && rank) arrive_leader<true>(&s.ready[slot]);
+        else mbar_arrive(&s.ready[slot]);
+        if (++slot == G::NST) {
+            slot = 0;
+            phase ^= 1u;
+        }
+    }
+}
+
 // ---- the kernel ---------------------------------------------------------------------
-template <bool HL, bool Q8>
-__global__ void __launch_bounds__(TILE_THREADS, 1) attn_tile_kernel(AttnTileArgs p, TilePlan pl) {
-    using G = TileGeo<HL>;
+template <bool HL, bool Q8, bool PAIR>
+__global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_kernel(AttnTileArgs p, TilePlan pl) {
+    using G = TileGeo<HL, Q8, PAIR>;
     using T = typename std::conditional<HL, float, __half>::type;
     extern __shared__ __align__(1024) uint8_t smem[];
     TileShared &s = *reinterpret_cast<TileShared *>(smem + G::SMEM);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t sbase = smem_u32(smem);
-    constexpr int MMA_WARP = SOFT_WARPS + LOAD_WARPS;
+    const int rank = PAIR ? (int)cta_rank() : 0;
+    constexpr int MMA_WARP = SOFT_WARPS + G::LOADERS;
     if (sbase & 1023u) {  // the swizzled layouts need 1024-byte aligned stages
         if (tid == 0) atomicOr(&g_dev_error, 256u);
         return;
     }
-
-    if (warp == 0) find_work(p, pl, s);
-    if (warp == MMA_WARP) tmem_alloc(&s.tmem, 512);
+    int work = 0;
+    if (warp == 0) work = find_work<G::CTAS, G::TK>(p, pl, s, rank);
     if (tid == 32) {
         for (int i = 0; i < G::NST; ++i) {
-            mbar_init(&s.full[i], LOAD_WARPS);
+            mbar_init(&s.full[i], G::LOADERS * 32);
             mbar_init(&s.empty[i], 1);
+            mbar_init(&s.ready[i], G::CTAS);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.s_full[i], 1);
-            mbar_init(&s.p_full[i], SOFT_WARPS);
+            mbar_init(&s.p_full[i], SOFT_WARPS * G::CTAS);
         }
         mbar_init(&s.pv_done, 1);
-        mbar_init(&s.q_full, SOFT_WARPS);
+        mbar_init(&s.q_full, SOFT_WARPS * G::CTAS);
+        mbar_init(&s.q_moved, SOFT_WARPS);
         mbar_init(&s.o_full, 1);
         s.abort = 0;
         fence_barrier_init();
     }
+    if (!__syncthreads_or(work)) return;
+    if (warp == MMA_WARP) tmem_take<PAIR>(&s.tmem);
     tc_fence_before();
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist
+    else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s.tmem;
 
-    if (s.nrow > 0 && warp >= SOFT_WARPS && warp < MMA_WARP) {
-        Loader<HL, Q8> ld{p, s, sbase + G::QB, tid - SOFT_WARPS * 32};
+    if (warp >= SOFT_WARPS && warp < MMA_WARP) {
+        Loader<HL, Q8, PAIR> ld{p, s, sbase + QBYTES, tid - SOFT_WARPS * 32, rank, s.lo, s.hi_max, s.end - s.begin};
         ld.run();
-    } else if (s.nrow > 0 && warp == MMA_WARP) {
-        if (lane == 0) {
-            Products<HL, Q8> mm{s, sbase, sbase + G::QB, tmem};
+    } else if (warp == MMA_WARP) {
+        if (rank == 0) {
+            Products<HL, Q8, PAIR> mm{s, sbase, sbase + QBYTES, tmem};
             mm.run();
         }
         __syncwarp();
-    } else if (s.nrow > 0) {
-        // softmax warps: row = TMEM lane, columns (positions, then dims) of one half
-        const int quarter = warp & 3, half = warp >> 2;
+    } else if (warp == MMA_WARP + 1) {
+        if (lane == 0) relay<HL, Q8, PAIR>(s, rank);
+        __syncwarp();
+    } else {
+        // softmax warps: row = TMEM lane; two groups of four, each a half of the columns (positions, then dims).
+        // (Groups that take whole tiles in turn overlap better with each other, but each then holds an S buffer
+        // twice as long, and with two buffers that is what the products wait for: 2.0 us a tile against 1.3.)
+        const int quarter = warp & 3, grp = warp >> 2;
         const int row = quarter * 32 + lane, tok = row / AGRP;
         const bool real = tok < s.nrow;
         const bool busy = quarter * 32 / AGRP < s.nrow;  // some row of this warp is real
-        const size_t grow = ((size_t)(s.row0 + (real ? tok : 0)) * AH + s.kvh * AGRP + row % AGRP);
         const int n = s.end - s.begin;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        auto head_row = [&](int r) { return (size_t)(s.row0 + r / AGRP) * AH + s.kvh * AGRP + r % AGRP; };
 
-        // stage Q: 16-byte pieces, 32 a row; a warp takes a row per pass
+        // stage Q: 16-byte pieces, 32 a row; a warp takes every eighth row, its loads first
         if (n > 0) {
-            const T *qg = static_cast<const T *>(p.q);
-            for (int r = warp; r < s.nrow * AGRP; r += SOFT_WARPS) {
-                const size_t at = ((size_t)(s.row0 + r / AGRP) * AH + s.kvh * AGRP + r % AGRP) * AHD + lane * 8;
-                const uint32_t dst = sbase + (lane >> 3) * 16384 + sw128_off(r, lane & 7);
-                if constexpr (HL) {
-                    const float4 a = *reinterpret_cast<const float4 *>(qg + at), b = *reinterpret_cast<const float4 *>(qg + at + 4);
-                    uint4 hi, lo;
-                    split2(a.x, a.y, hi.x, lo.x);
-                    split2(a.z, a.w, hi.y, lo.y);
-                    split2(b.x, b.y, hi.z, lo.z);
-                    split2(b.z, b.w, hi.w, lo.w);
-                    sts16(dst, hi);
-                    sts16(dst + QBYTES, lo);
-                } else {
-                    sts16(dst, *reinterpret_cast<const uint4 *>(qg + at));
+            const T *qg = static_cast<const T *>(p.q) + lane * 8;
+            const uint32_t qlo = sbase + G::SMEM - QBYTES;
+            constexpr int NB = HL ? 8 : 16;  // rows a batch
+            for (int r0 = warp; r0 < s.nrow * AGRP; r0 += SOFT_WARPS * NB) {
+                uint4 v[16];
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    const int r = r0 + i * SOFT_WARPS;
+                    if (r < s.nrow * AGRP) {
+                        const uint4 *src = reinterpret_cast<const uint4 *>(qg + head_row(r) * AHD);
+                        if constexpr (HL) {
+                            v[2 * i] = src[0];
+                            v[2 * i + 1] = src[1];
+                        } else {
+                            v[i] = src[0];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    const int r = r0 + i * SOFT_WARPS;
+                    if (r >= s.nrow * AGRP) break;
+                    const uint32_t dst = (lane >> 3) * 16384 + sw128_off(r, lane & 7);
+                    if constexpr (HL) {
+                        const float4 x = *reinterpret_cast<const float4 *>(&v[2 * i]), y = *reinterpret_cast<const float4 *>(&v[2 * i + 1]);
+                        uint4 hi, lo;
+                        split2(x.x, x.y, hi.x, lo.x);
+                        split2(x.z, x.w, hi.y, lo.y);
+                        split2(y.x, y.y, hi.z, lo.z);
+                        split2(y.z, y.w, hi.w, lo.w);
+                        sts16(sbase + dst, hi);
+                        sts16(qlo + dst, lo);
+                    } else {
+                        sts16(sbase + dst, v[i]);
+                    }
                 }
             }
             fence_async_smem();
+            if constexpr (HL) {
+                named_sync(9, SOFT_WARPS * 32);
+                if (busy) {
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {  // 32 dims: 16 columns
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int c = grp * 16 + b * 4 + i;
+                            lds16(qlo + (c >> 3) * 16384 + sw128_off(row, c & 7), w + 4 * i);
+                        }
+                        tmem_st16(tmem + lanes + kQlo + grp * 64 + b * 16, w);
+                    }
+                    tmem_st_wait();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s.q_moved);
+            }
+            tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s.q_full);
+            if (lane == 0) {
+                if (PAIR && rank) arrive_leader<true>(&s.q_full);
+                else mbar_arrive(&s.q_full);
+            }
         }
 
         const float c = p.scale * kLog2e;
         const int hi = real ? s.hi[tok] : 0x7fffffff, sk = real ? s.sk[tok] : 0, rs = real ? s.rs[tok] : 0;
         float m = -INFINITY, l = 0.0f;  // maximum in use; sum of this half's columns
+        constexpr int CW = G::TK / 2, NB = CW / 32;
         for (int j = 0; j < n; ++j) {
-            const uint32_t sb = tmem + lanes + 256 + (j & 1) * 128;
+            const uint32_t sb = tmem + lanes + G::S0 + (j & 1) * G::TK;
             tw(&s.s_full[j & 1], (uint32_t)(j >> 1) & 1u, s, 32u);
             tc_fence_after();
             if (busy) {
-                uint32_t u[64];
-                tmem_ld32_async(sb + half * 64, u);
-                tmem_ld32_async(sb + half * 64 + 32, u + 32);
-                tmem_ld_wait();
-                float f[64];
+                const int pos0 = tile_at(s, s.begin + j) * G::TK;
+                const bool cut = pos0 < s.lo || pos0 + G::TK > s.hi_min || pos0 < s.rs_max;  // some row does not see all of it
+                const int lo = s.lo;
+                uint32_t u[NB][32];
+                float mx = -INFINITY;
+                tmem_ld32_async(sb + grp * CW, u[0]);
 #pragma unroll
-                for (int i = 0; i < 64; ++i) f[i] = __uint_as_float(u[i]);
-                const int t = tile_at(s, s.begin + j), pos0 = t * TK;
-                if (pos0 < s.lo || pos0 + TK > s.hi_min || pos0 < s.rs_max) {  // some row does not see all of the tile
-                    const int lo = s.lo;
+                for (int b = 0; b < NB; ++b) {
+                    tmem_ld_wait();
+                    if (b + 1 < NB) tmem_ld32_async(sb + grp * CW + (b + 1) * 32, u[b + 1]);
+                    if (cut) {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        const int pos = pos0 + half * 64 + i;
-                        if (pos >= hi || pos < lo || (pos >= sk && pos < rs)) f[i] = -INFINITY;
+                        for (int i = 0; i < 32; ++i) {
+                            const int pos = pos0 + grp * CW + b * 32 + i;
+                            if (pos >= hi || pos < lo || (pos >= sk && pos < rs)) u[b][i] = 0xff800000u;  // -inf
+                        }
                     }
-                }
-                float mx = f[0];
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 1; i < 64; ++i) mx = fmaxf(mx, f[i]);
-                s.ex[j & 1][half][row] = mx;
+                    for (int i = 0; i < 32; ++i) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(u[b][i]));
+                    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                }
+                s.ex[j & 1][grp][row] = mx;
                 named_sync(1 + quarter, 64);  // also: both halves have read S, P may overwrite it
-                mx = fmaxf(mx, s.ex[j & 1][half ^ 1][row]);
-                const bool grow_m = mx > m && (m == -INFINITY || (mx - m) * c > kSlack);
-                if (__any_sync(0xffffffffu, grow_m)) {
-                    const float nm = grow_m ? mx : m;
+                mx = fmaxf(mx, s.ex[j & 1][grp ^ 1][row]);
+                const bool grow = mx > m && (m == -INFINITY || (mx - m) * c > kSlack);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float nm = grow ? mx : m;
                     const float alpha = m == -INFINITY ? 0.0f : ex2((m - nm) * c);
                     if (j > 0) {
                         tw(&s.pv_done, (uint32_t)(j - 1) & 1u, s, 64u);
@@ -515,7 +804,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) attn_tile_kernel(AttnTileArgs
 #pragma unroll
                         for (int b = 0; b < 8; ++b) {
                             uint32_t o[16];
-                            const uint32_t ob = tmem + lanes + half * 128 + b * 16;
+                            const uint32_t ob = tmem + lanes + grp * 128 + b * 16;
                             tmem_ld16_async(ob, o);
                             tmem_ld_wait();
 #pragma unroll
@@ -528,97 +817,93 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) attn_tile_kernel(AttnTileArgs
                 }
                 const float off = m == -INFINITY ? 0.0f : fmaf(m, c, -kShift);
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    uint32_t h[16], w[16];
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t h[16];
+                    [[maybe_unused]] uint32_t w[16];
+                    float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float e0 = ex2(fmaf(f[32 * b + 2 * i], c, -off)), e1 = ex2(fmaf(f[32 * b + 2 * i + 1], c, -off));
-                        l += e0 + e1;
+                        const float e0 = ex2(fmaf(__uint_as_float(u[b][2 * i]), c, -off));
+                        const float e1 = ex2(fmaf(__uint_as_float(u[b][2 * i + 1]), c, -off));
+                        l0 += e0;
+                        l1 += e1;
                         if constexpr (HL) split2(e0, e1, h[i], w[i]);
                         else h[i] = pack2(e0, e1);
                     }
-                    tmem_st16(sb + half * 32 + b * 16, h);
-                    if constexpr (HL) tmem_st16(sb + 64 + half * 32 + b * 16, w);
+                    l += l0 + l1;
+                    tmem_st16(sb + grp * (CW / 2) + b * 16, h);
+                    if constexpr (HL) tmem_st16(sb + CW + grp * (CW / 2) + b * 16, w);
                 }
                 tmem_st_wait();
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s.p_full[j & 1]);
+            if (lane == 0) {
+                if (PAIR && rank) arrive_leader<false>(&s.p_full[j & 1]);
+                else mbar_arrive(&s.p_full[j & 1]);
+            }
         }
+
+        // O, scaled, to rows of the (free) ring; from there coalesced
         if (n > 0) {
             tw(&s.o_full, 0, s, 128u);
             tc_fence_after();
         }
+        const int parts = pl.ns + pl.ns_own;
+        const bool join = parts > 1;
+        float *buf = reinterpret_cast<float *>(smem);
+        constexpr int BROW = AHD + 4;  // floats; 16-byte stores of 8 rows hit distinct banks
         if (busy) {
-            s.ex[n & 1][half][row] = l;
+            s.ex[n & 1][grp][row] = l;
             named_sync(1 + quarter, 64);
-            l += s.ex[n & 1][half ^ 1][row];
-            const bool join = pl.ns + pl.ns_own > 1;
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            const int parts = pl.ns + pl.ns_own;
-            const size_t slot = grow * parts + s.part;
-            float2 *ml = static_cast<float2 *>(p.ws);
-            float *acc = reinterpret_cast<float *>(ml + (size_t)p.n_row * AH * parts) + slot * AHD + half * 128;
-            T *out = static_cast<T *>(p.out) + grow * AHD + half * 128;
-            const T *gate = p.gate ? static_cast<const T *>(p.gate) + grow * AHD + half * 128 : nullptr;
-            if (join && real && half == 0) ml[slot] = make_float2(m == -INFINITY ? m : fmaf(m, c, -kShift), l);
+            l += s.ex[n & 1][grp ^ 1][row];
+            const float inv = join ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
+            if (n > 0) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                uint32_t o[32];
-                if (n > 0) {
-                    tmem_ld32_async(tmem + lanes + half * 128 + b * 32, o);
+                for (int b = 0; b < 4; ++b) {
+                    uint32_t o[32];
+                    tmem_ld32_async(tmem + lanes + grp * 128 + b * 32, o);
                     tmem_ld_wait();
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0u;
-                }
-                if (!real) continue;
-                if (join) {
-                    if (n > 0) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4 *>(acc + b * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    }
-                    continue;
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(o[i + e]) * inv;
-                    if constexpr (HL) {
-                        if (gate) {
-                            const float4 ga = *reinterpret_cast<const float4 *>(gate + b * 32 + i), gb = *reinterpret_cast<const float4 *>(gate + b * 32 + i + 4);
-                            const float g[8] = {ga.x, ga.y, ga.z, ga.w, gb.x, gb.y, gb.z, gb.w};
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) y[e] *= sigmoid_f(g[e]);
-                        }
-                        *reinterpret_cast<float4 *>(out + b * 32 + i) = make_float4(y[0], y[1], y[2], y[3]);
-                        *reinterpret_cast<float4 *>(out + b * 32 + i + 4) = make_float4(y[4], y[5], y[6], y[7]);
-                    } else {
-                        if (gate) {
-                            const uint4 gw = *reinterpret_cast<const uint4 *>(gate + b * 32 + i);
-                            const __half2 *gh = reinterpret_cast<const __half2 *>(&gw);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float2 g = __half22float2(gh[e]);
-                                y[2 * e] *= sigmoid_f(g.x);
-                                y[2 * e + 1] *= sigmoid_f(g.y);
-                            }
-                        }
-                        *reinterpret_cast<uint4 *>(out + b * 32 + i) =
-                            make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
-                    }
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4 *>(buf + row * BROW + grp * 128 + b * 32 + i) =
+                            make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
+                                        __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
                 }
             }
+            if (join && real && grp == 0)
+                static_cast<float2 *>(p.ws)[head_row(row) * parts + s.part] = make_float2(m == -INFINITY ? m : fmaf(m, c, -kShift), l);
+        }
+        named_sync(9, SOFT_WARPS * 32);
+        float *acc = reinterpret_cast<float *>(static_cast<float2 *>(p.ws) + (size_t)p.n_row * AH * parts);
+#pragma unroll 4
+        for (int r = warp; r < s.nrow * AGRP; r += SOFT_WARPS) {
+            const size_t g = head_row(r);
+            float y[8] = {};
+            if (n > 0) {
+                const float4 x0 = *reinterpret_cast<const float4 *>(buf + r * BROW + lane * 8);
+                const float4 x1 = *reinterpret_cast<const float4 *>(buf + r * BROW + lane * 8 + 4);
+                y[0] = x0.x; y[1] = x0.y; y[2] = x0.z; y[3] = x0.w; y[4] = x1.x; y[5] = x1.y; y[6] = x1.z; y[7] = x1.w;
+            }
+            if (join) {
+                if (n > 0) put8(acc + (g * parts + s.part) * AHD + lane * 8, y);
+                continue;
+            }
+            if (p.gate) {
+                float gv[8];
+                get8(static_cast<const T *>(p.gate) + g * AHD + lane * 8, gv);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] *= sigmoid_f(gv[i]);
+            }
+            put8(static_cast<T *>(p.out) + g * AHD + lane * 8, y);
         }
     }
     tc_fence_before();
-    __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // (also: no CTA leaves while the other may still signal it)
+    else __syncthreads();
     if (warp == MMA_WARP) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_give<PAIR>(tmem);
     }
 }
 
@@ -643,29 +928,28 @@ __global__ void __launch_bounds__(AH * 32) attn_join_kernel(AttnTileArgs p, int 
             l = fmaf(w, t.y, l);
         }
         const int n = min(32, parts - i0);
+#pragma unroll 4
         for (int i = 0; i < n; ++i) {
             const float wi = __shfl_sync(0xffffffffu, w, i);
-            if (wi == 0.0f) continue;
-            const float4 a = *reinterpret_cast<const float4 *>(acc + (size_t)(i0 + i) * AHD);
-            const float4 b = *reinterpret_cast<const float4 *>(acc + (size_t)(i0 + i) * AHD + 4);
+            float4 a = make_float4(0, 0, 0, 0), b = a;
+            if (wi != 0.0f) {  // (an empty part has no values)
+                a = *reinterpret_cast<const float4 *>(acc + (size_t)(i0 + i) * AHD);
+                b = *reinterpret_cast<const float4 *>(acc + (size_t)(i0 + i) * AHD + 4);
+            }
             o[0] = fmaf(wi, a.x, o[0]); o[1] = fmaf(wi, a.y, o[1]); o[2] = fmaf(wi, a.z, o[2]); o[3] = fmaf(wi, a.w, o[3]);
             o[4] = fmaf(wi, b.x, o[4]); o[5] = fmaf(wi, b.y, o[5]); o[6] = fmaf(wi, b.z, o[6]); o[7] = fmaf(wi, b.w, o[7]);
         }
     }
     l = warp_sum(l);
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    T *out = static_cast<T *>(p.out) + g * AHD + lane * 8;
+    float gv[8];
+    if (p.gate) get8(static_cast<const T *>(p.gate) + g * AHD + lane * 8, gv);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         o[i] *= inv;
-        if (p.gate) o[i] *= sigmoid_f(to_f32(static_cast<const T *>(p.gate)[g * AHD + lane * 8 + i]));
+        if (p.gate) o[i] *= sigmoid_f(gv[i]);
     }
-    if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(out) = make_float4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<float4 *>(out + 4) = make_float4(o[4], o[5], o[6], o[7]);
-    } else {
-        *reinterpret_cast<uint4 *>(out) = make_uint4(pack2(o[0], o[1]), pack2(o[2], o[3]), pack2(o[4], o[5]), pack2(o[6], o[7]));
-    }
+    put8(static_cast<T *>(p.out) + g * AHD + lane * 8, o);
 }
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -673,19 +957,21 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // The same plan for the workspace query and the launch.
 TilePlan plan_for(int n_row, int n_run, int max_run, int max_len, int max_own, bool shared) {
     TilePlan pl{};
-    pl.tiles = n_row / TM_TOK + (n_run < n_row ? n_run : n_row);
+    pl.pair = !shared && max_run > TM_TOK;
+    const int toks = TM_TOK * (pl.pair ? 2 : 1), sms = kPlanSMs / (pl.pair ? 2 : 1);
+    pl.tiles = n_row / toks + (n_run < n_row ? n_run : n_row);
     if (!shared) {
-        const long long most = (long long)n_run * ceil_div(max_run, TM_TOK);
+        const long long most = (long long)n_run * ceil_div(max_run, toks);
         if (most < pl.tiles) pl.tiles = (int)most;
-        const int units = pl.tiles * AKV, kv = ceil_div(max_len, TK);
-        pl.ns = units >= kPlanSMs ? 1 : kPlanSMs / units;
+        const int units = pl.tiles * AKV, kv = ceil_div(max_len, kPlanTile);
+        pl.ns = units >= sms ? 1 : sms / units;
         if (pl.ns > kv) pl.ns = kv;
         return pl;
     }
     // shared prefixes: parts of equal length, one wave of CTAs at most for the prefixes
-    const int kv = ceil_div(max_len, TK), kv_own = ceil_div(max_own, TK) + 1;
+    const int kv = ceil_div(max_len, kPlanTile), kv_own = ceil_div(max_own, kPlanTile) + 1;
     const long long work = (long long)AKV * ((long long)pl.tiles * kv + (long long)n_row * kv_own);
-    int each = ceil_div(work, kPlanSMs);
+    const int each = ceil_div(work, kPlanSMs);
     pl.ns = kv > 0 ? ceil_div(kv, each) : 1;
     pl.own_tiles = n_row;
     pl.ns_own = ceil_div(kv_own, each);
@@ -697,17 +983,35 @@ size_t parts_bytes(int n_row, const TilePlan &pl) {
     return parts > 1 ? (size_t)n_row * AH * parts * (sizeof(float2) + AHD * sizeof(float)) : 256;
 }
 
-template <bool HL, bool Q8>
+template <bool HL, bool Q8, bool PAIR>
 cudaError_t launch_tile(const AttnTileArgs &a, const TilePlan &pl, cudaStream_t st) {
-    auto kern = attn_tile_kernel<HL, Q8>;
-    constexpr int smem = (int)(TileGeo<HL>::SMEM + sizeof(TileShared));
+    using G = TileGeo<HL, Q8, PAIR>;
+    auto kern = attn_tile_kernel<HL, Q8, PAIR>;
+    constexpr int smem = (int)(G::SMEM + sizeof(TileShared));
     static_assert(smem <= 227 * 1024, "stages and Q fit one SM");
+    static_assert(G::NST <= kMaxStages, "a barrier for every stage");
     cudaError_t e = qw35h::smem_optin((const void *)kern, smem);
     if (e != cudaSuccess) return e;
-    const long long grid = (long long)pl.tiles * AKV * pl.ns + (long long)pl.own_tiles * AKV * pl.ns_own;
+    const long long grid = G::CTAS * ((long long)pl.tiles * AKV * pl.ns + (long long)pl.own_tiles * AKV * pl.ns_own);
     if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-    kern<<<(unsigned)grid, TILE_THREADS, smem, st>>>(a, pl);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(G::THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = G::CTAS;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, a, pl);
+}
+
+template <bool PAIR>
+cudaError_t launch_type(const AttnTileArgs &a, const TilePlan &pl, cudaStream_t st) {
+    return a.half ? (a.kv_q8 ? launch_tile<false, true, PAIR>(a, pl, st) : launch_tile<false, false, PAIR>(a, pl, st))
+                  : (a.kv_q8 ? launch_tile<true, true, PAIR>(a, pl, st) : launch_tile<true, false, PAIR>(a, pl, st));
 }
 
 }  // namespace
@@ -720,8 +1024,7 @@ cudaError_t attn_tile_run(const AttnTileArgs &a, cudaStream_t st) {
     if (a.n_row <= 0) return cudaSuccess;
     const TilePlan pl = plan_for(a.n_row, a.n_run, a.max_run, a.max_len, a.max_own, a.shared_len != nullptr);
     if (a.ws_bytes < parts_bytes(a.n_row, pl)) return cudaErrorInvalidValue;
-    cudaError_t e = a.half ? (a.kv_q8 ? launch_tile<false, true>(a, pl, st) : launch_tile<false, false>(a, pl, st))
-                           : (a.kv_q8 ? launch_tile<true, true>(a, pl, st) : launch_tile<true, false>(a, pl, st));
+    cudaError_t e = pl.pair ? launch_type<true>(a, pl, st) : launch_type<false>(a, pl, st);
     if (e != cudaSuccess) return e;
     const int parts = pl.ns + pl.ns_own;
     if (parts > 1) {
