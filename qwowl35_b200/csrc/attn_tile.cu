@@ -20,14 +20,15 @@
 // What the ring holds decides the speed: a V tile waits in it for its softmax,
 // and the rest has to cover the latency of L2 or HBM.  Hence
 //   single CTAs   64 positions a tile; 5 stages of 32 KB beside Q (64 KB);
-//   CTA pairs     (runs of more than 32 tokens) 256 rows share one K/V tile, each
-//                 CTA holding half of it (cta_group::2): half the L2 reads and
-//                 twice the tiles in the ring.  128 positions a tile in f16.
+//   CTA pairs     (runs of more than 32 tokens) 256 rows share one K/V tile of
+//                 128 positions, each CTA holding half of it (cta_group::2): half
+//                 the L2 reads and twice the tiles in the ring.
 // f32 calls (HL) carry q and p as f16 hi + lo pairs, two products each, ~22
-// bits; Q's lo half sits in TMEM, where 64-position S buffers leave 128 columns,
-// so that the ring keeps its size.  q8_0 values d * code (18 bits) then enter as
-// hi + lo stages as well.  f16 calls round p to f16 once, and q8_0 values once,
-// the rounding their type implies.
+// bits.  Q's lo half sits in TMEM for single CTAs, where 64-position S buffers
+// leave 128 columns and the ring keeps its size; for pairs, bound by the products
+// and so better off with 128 positions a product, beside Q (3 stages remain).
+// q8_0 values d * code (18 bits) then enter as hi + lo stages as well.  f16 calls
+// round p to f16 once, and q8_0 values once, the rounding their type implies.
 //
 // The running maximum is lazy: O is rescaled only when a row's maximum grows by
 // more than 2^8 over the one in use, so P reaches at most 2^15 (its 2^7 offset
@@ -35,6 +36,7 @@
 //
 // Work is split along the positions where there are few row tiles; the parts'
 // (m, l, O) go through the workspace and attn_join_kernel merges them.
+#include <cstdlib>
 #include <type_traits>
 
 #include "kvcache.cuh"
@@ -57,20 +59,22 @@ constexpr float kShift = 7.0f, kSlack = 8.0f;  // log2: offset of P, growth of t
 template <bool HL, bool Q8, bool PAIR>
 struct TileGeo {
     static constexpr int CTAS = PAIR ? 2 : 1;
-    static constexpr int TK = PAIR && !HL ? 128 : 64;    // positions of a tile; divides a chunk
+    static constexpr int TK = PAIR ? 128 : 64;           // positions of a tile; divides a chunk
     static constexpr int KR = TK / CTAS;                 // positions of K a CTA holds
     static constexpr int VP = 32 / CTAS;                 // 16-byte pieces of a V row a CTA holds
     static constexpr uint32_t STAGE = (uint32_t)TK * AHD * 2 / CTAS;
-    static constexpr int NST = 5 * 32768 / (int)STAGE;   // what 227 KB hold beside Q
+    static constexpr bool LO_SMEM = HL && PAIR, LO_TMEM = HL && !PAIR;  // where Q's lo half is
+    static constexpr uint32_t QB = LO_SMEM ? 2 * QBYTES : QBYTES;
+    static constexpr int NST = LO_SMEM ? 3 : 5;          // stages: what 227 KB hold beside Q
     // f16 planes: four warps issue the copies; q8_0: six convert, as many as fit 16 warps of 128 registers
     static constexpr int LOADERS = Q8 ? 6 : 4;
     static constexpr int THREADS = (SOFT_WARPS + LOADERS + 2) * 32;
-    [[maybe_unused]] static constexpr int WSTEPS = (int)STAGE / 512, STEPS = (WSTEPS + LOADERS - 1) / LOADERS;  // q8_0: a warp's passes over a stage
+    enum : int { WSTEPS = STAGE / 512, STEPS = (WSTEPS + LOADERS - 1) / LOADERS };  // q8_0: passes over a stage, of a warp
     static constexpr int PARTS = HL && Q8 ? 2 : 1;       // stages of a tile: values, or their hi and lo halves
-    static constexpr uint32_t RING = NST * STAGE, SMEM = QBYTES + RING;
-    static constexpr uint32_t S0 = 256;       // TMEM columns
-    // f32: Q's lo half passes through the last 64 KB of the ring on its way to TMEM
-    static constexpr int FREE_AT_START = HL ? (int)((RING - QBYTES) / STAGE) : NST;
+    static constexpr uint32_t RING = NST * STAGE, SMEM = QB + RING;
+    static constexpr uint32_t S0 = 256;                  // TMEM columns: O, then the S buffers, then (LO_TMEM) Q's lo half
+    // a lo half bound for TMEM passes through the last 64 KB of the ring
+    static constexpr int FREE_AT_START = LO_TMEM ? (int)((RING - QBYTES) / STAGE) : NST;
 };
 
 struct TilePlan {
@@ -82,7 +86,7 @@ struct TilePlan {
 };
 
 constexpr uint32_t kQlo = 384;  // TMEM columns of the lo half of Q
-constexpr int kMaxStages = 10;
+constexpr int kMaxStages = 5;
 struct __align__(16) TileShared {
     uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages];
     uint64_t s_full[2], p_full[2], pv_done, q_full, q_moved, o_full;
@@ -219,6 +223,9 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo = pack2(a - f.x, b - f.y);
 }
 
+// 1 / (1 + e^-x), a few units of 2^-24 off (sigmoid_f's exact division and exponential cost an epilogue 4 us)
+__device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.0f, 1.0f + ex2(fmaxf(-x * kLog2e, -126.0f))); }
+
 // 8 consecutive values of a row, 16-byte aligned
 __device__ __forceinline__ void get8(const float *p, float *v) {
     const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
@@ -255,12 +262,18 @@ __device__ __forceinline__ int run_of_row(const AttnTileArgs &p, int r) {
     return n > 0 && r < p.off[n] ? n - 1 : -1;
 }
 
-// Row tile `tile` -> its run and first row, by one converged warp; false behind the last tile.
-__device__ __forceinline__ bool find_tile(const AttnTileArgs &p, int tile, int toks, int &run, int &row0) {
+struct RunRows {
+    int run, begin, end, len, row0;  // run (group), its rows, len[run] (or shared_len[run]), the tile's first row
+};
+// Row tile `tile` of `toks` rows -> its run, by one converged warp; run = -1 behind the last tile.  What is needed of
+// a run is loaded in one go: the latency counts, not the bytes.
+__device__ __forceinline__ RunRows find_tile(const AttnTileArgs &p, int tile, int toks) {
     const int lane = threadIdx.x & 31;
+    const int32_t *lens = p.shared_len ? p.shared_len : p.len;
     int before = 0;
     for (int u = 0; u < p.n_run; u += 32) {
-        const int a = u + lane < p.n_run ? p.off[u + lane] : 0, b = u + lane < p.n_run ? p.off[u + lane + 1] : 0;
+        const bool in = u + lane < p.n_run;
+        const int a = in ? p.off[u + lane] : 0, b = in ? p.off[u + lane + 1] : 0, len = in ? lens[u + lane] : 0;
         const int n = b > a ? (b - a + toks - 1) / toks : 0;
         int sum = n;
 #pragma unroll
@@ -271,37 +284,43 @@ __device__ __forceinline__ bool find_tile(const AttnTileArgs &p, int tile, int t
         const unsigned hit = __ballot_sync(0xffffffffu, before + sum > tile);
         if (hit) {
             const int w = __ffs(hit) - 1;
-            run = u + w;
-            row0 = __shfl_sync(0xffffffffu, a + (tile - (before + sum - n)) * toks, w);
-            return true;
+            const int first = a + (tile - (before + sum - n)) * toks;
+            return RunRows{u + w, __shfl_sync(0xffffffffu, a, w), __shfl_sync(0xffffffffu, b, w),
+                           __shfl_sync(0xffffffffu, len, w), __shfl_sync(0xffffffffu, first, w)};
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    return false;
+    return RunRows{-1, 0, 0, 0, 0};
 }
 
 // What this CTA does, by warp 0; false when there is no such unit (for both CTAs of a pair).
 template <int CTAS, int TK>
 __device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan &pl, TileShared &s, int rank) {
     const int lane = threadIdx.x & 31;
-    int id = blockIdx.x / CTAS, run = -1, row0 = 0, nrow = 0, ns = pl.ns, split, kvh;
+    int id = blockIdx.x / CTAS, nrow = 0, ns = pl.ns, split, kvh;
     const int n_first = pl.tiles * AKV * pl.ns;
     const bool tail = id >= n_first;
+    RunRows w{-1, 0, 0, 0, 0};
     if (!tail) {
         split = id % ns;
         kvh = (id / ns) % AKV;
         int tile = id / (AKV * ns);
         if (!p.shared_len) tile = pl.tiles - 1 - tile;  // the last tokens of a run have the most to do: first
-        if (find_tile(p, tile, TM_TOK * CTAS, run, row0)) nrow = min(TM_TOK * CTAS, p.off[run + 1] - row0);
+        w = find_tile(p, tile, TM_TOK * CTAS);
+        if (w.run >= 0) nrow = min(TM_TOK * CTAS, w.end - w.row0);
     } else {
         id -= n_first;
         ns = pl.ns_own;
         split = id % ns;
         kvh = (id / ns) % AKV;
-        row0 = id / (AKV * ns);
-        run = run_of_row(p, row0);
-        nrow = run >= 0 ? 1 : 0;
+        w.row0 = id / (AKV * ns);
+        w.run = run_of_row(p, w.row0);
+        if (w.run >= 0) {
+            nrow = 1;
+            w.len = p.shared_len[w.run];
+        }
     }
+    const int row0 = w.row0;
     if (row0 < 0 || row0 + nrow > p.n_row) nrow = 0;
     // lane = token of the CTA's tile; a pair walks the positions that either of its tiles needs
     int lo = 0, hi_max = 0, rs_min = 0x7fffffff, sk_max = 0;
@@ -311,13 +330,13 @@ __device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan 
         int hi = 0, sk = 0, rs = 0;
         if (real) {
             const int r = row0 + tok;
-            int L = p.shared_len ? p.len[r] : p.len[run] - (p.off[run + 1] - p.off[run]) + (r - p.off[run]) + 1;
+            int L = p.shared_len ? p.len[r] : w.len - (w.end - r) + 1;
             L = max(0, min(L, p.max_chunks * ACHUNK));
             int total;
             attended_range(L, p.window, p.sink, total, sk, rs);
             hi = L;
             if (p.shared_len) {
-                const int sh = max(0, p.shared_len[run]);
+                const int sh = max(0, w.len);
                 if (tail) lo = sh;
                 else hi = min(L, sh);
             }
@@ -350,7 +369,7 @@ __device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan 
         s.row0 = row0 + rank * TM_TOK;
         s.nrow = max(0, min(TM_TOK, nrow - rank * TM_TOK));
         s.kvh = kvh;
-        s.table = p.shared_len ? (tail ? row0 : (run >= 0 ? p.off[run] : 0)) : max(run, 0);
+        s.table = p.shared_len ? (tail ? row0 : w.begin) : max(w.run, 0);
         s.part = tail ? pl.ns + split : split;
         s.lo = lo; s.hi_max = hi_max;
         s.a0 = a0; s.n1 = n1; s.t2 = t2;
@@ -558,7 +577,10 @@ struct Products {
         if (elect_one()) {
             if constexpr (HL) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mma_ts<PAIR>(d, tmem + kQlo + i * 8, kd0 + kstep(i), idesc, i > 0);
+                for (int i = 0; i < 16; ++i) {
+                    if constexpr (G::LO_TMEM) mma_ts<PAIR>(d, tmem + kQlo + i * 8, kd0 + kstep(i), idesc, i > 0);
+                    else mma_ss<PAIR>(d, qd + (QBYTES >> 4) + qstep(i), kd0 + kstep(i), idesc, i > 0);
+                }
                 if constexpr (Q8) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) mma_ss<PAIR>(d, qd + qstep(i), kd1 + kstep(i), idesc, 1);
@@ -662,6 +684,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
         s.abort = 0;
         fence_barrier_init();
     }
+    pdl_trigger();
     if (!__syncthreads_or(work)) return;
     if (warp == MMA_WARP) tmem_take<PAIR>(&s.tmem);
     tc_fence_before();
@@ -671,11 +694,11 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
     const uint32_t tmem = s.tmem;
 
     if (warp >= SOFT_WARPS && warp < MMA_WARP) {
-        Loader<HL, Q8, PAIR> ld{p, s, sbase + QBYTES, tid - SOFT_WARPS * 32, rank, s.lo, s.hi_max, s.end - s.begin};
+        Loader<HL, Q8, PAIR> ld{p, s, sbase + G::QB, tid - SOFT_WARPS * 32, rank, s.lo, s.hi_max, s.end - s.begin};
         ld.run();
     } else if (warp == MMA_WARP) {
         if (rank == 0) {
-            Products<HL, Q8, PAIR> mm{s, sbase, sbase + QBYTES, tmem};
+            Products<HL, Q8, PAIR> mm{s, sbase, sbase + G::QB, tmem};
             mm.run();
         }
         __syncwarp();
@@ -697,7 +720,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
         // stage Q: 16-byte pieces, 32 a row; a warp takes every eighth row, its loads first
         if (n > 0) {
             const T *qg = static_cast<const T *>(p.q) + lane * 8;
-            const uint32_t qlo = sbase + G::SMEM - QBYTES;
+            const uint32_t qlo = sbase + (G::LO_TMEM ? G::SMEM - QBYTES : QBYTES);
             constexpr int NB = HL ? 8 : 16;  // rows a batch
             for (int r0 = warp; r0 < s.nrow * AGRP; r0 += SOFT_WARPS * NB) {
                 uint4 v[16];
@@ -734,7 +757,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 }
             }
             fence_async_smem();
-            if constexpr (HL) {
+            if constexpr (G::LO_TMEM) {
                 named_sync(9, SOFT_WARPS * 32);
                 if (busy) {
 #pragma unroll
@@ -844,13 +867,29 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
             }
         }
 
-        // O, scaled, to rows of the (free) ring; from there coalesced
+        // O goes, scaled, to rows of the (free) ring and from there out coalesced, a warp per row; the gates of the
+        // first rows are fetched before the last product ends
+        const int parts = pl.ns + pl.ns_own, rows = s.nrow * AGRP;
+        const bool join = parts > 1;
+        constexpr int EB = HL ? 4 : 8;  // rows a batch
+        uint4 gates[EB][HL ? 2 : 1];
+        auto fetch_gates = [&](int r0) {
+            if (!p.gate || join) return;
+#pragma unroll
+            for (int i = 0; i < EB; ++i) {
+                const int r = r0 + i * SOFT_WARPS;
+                if (r < rows) {
+                    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.gate) + head_row(r) * AHD + lane * 8);
+                    gates[i][0] = src[0];
+                    if constexpr (HL) gates[i][1] = src[1];
+                }
+            }
+        };
+        fetch_gates(warp);
         if (n > 0) {
             tw(&s.o_full, 0, s, 128u);
             tc_fence_after();
         }
-        const int parts = pl.ns + pl.ns_own;
-        const bool join = parts > 1;
         float *buf = reinterpret_cast<float *>(smem);
         constexpr int BROW = AHD + 4;  // floats; 16-byte stores of 8 rows hit distinct banks
         if (busy) {
@@ -876,26 +915,27 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
         }
         named_sync(9, SOFT_WARPS * 32);
         float *acc = reinterpret_cast<float *>(static_cast<float2 *>(p.ws) + (size_t)p.n_row * AH * parts);
-#pragma unroll 4
-        for (int r = warp; r < s.nrow * AGRP; r += SOFT_WARPS) {
-            const size_t g = head_row(r);
-            float y[8] = {};
-            if (n > 0) {
-                const float4 x0 = *reinterpret_cast<const float4 *>(buf + r * BROW + lane * 8);
-                const float4 x1 = *reinterpret_cast<const float4 *>(buf + r * BROW + lane * 8 + 4);
-                y[0] = x0.x; y[1] = x0.y; y[2] = x0.z; y[3] = x0.w; y[4] = x1.x; y[5] = x1.y; y[6] = x1.z; y[7] = x1.w;
-            }
-            if (join) {
-                if (n > 0) put8(acc + (g * parts + s.part) * AHD + lane * 8, y);
-                continue;
-            }
-            if (p.gate) {
-                float gv[8];
-                get8(static_cast<const T *>(p.gate) + g * AHD + lane * 8, gv);
+        for (int r0 = warp; r0 < rows; r0 += SOFT_WARPS * EB) {
+            if (r0 != warp) fetch_gates(r0);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] *= sigmoid_f(gv[i]);
+            for (int i = 0; i < EB; ++i) {
+                const int r = r0 + i * SOFT_WARPS;
+                if (r >= rows) break;
+                const size_t g = head_row(r);
+                float y[8] = {};
+                if (n > 0) get8(buf + r * BROW + lane * 8, y);
+                if (join) {
+                    if (n > 0) put8(acc + (g * parts + s.part) * AHD + lane * 8, y);
+                    continue;
+                }
+                if (p.gate) {
+                    float gv[8];
+                    get8(reinterpret_cast<const T *>(&gates[i][0]), gv);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] *= sigmoid_fast(gv[e]);
+                }
+                put8(static_cast<T *>(p.out) + g * AHD + lane * 8, y);
             }
-            put8(static_cast<T *>(p.out) + g * AHD + lane * 8, y);
         }
     }
     tc_fence_before();
@@ -907,12 +947,20 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
     }
 }
 
-// Merges the parts of each (row, head): a warp per head, 8 dims a lane.
+// Merges the parts of a (row, head): four warps take every fourth part, 8 dims a lane.  The loads of a warp's
+// parts go out eight at a time: with few rows their latency is all there is.
+constexpr int JOIN_WARPS = 4;
 template <typename T>
-__global__ void __launch_bounds__(AH * 32) attn_join_kernel(AttnTileArgs p, int parts) {
-    const int row = blockIdx.x, lane = threadIdx.x & 31, h = threadIdx.x >> 5;
-    if (run_of_row(p, row) < 0) return;
+__global__ void __launch_bounds__(JOIN_WARPS * 32) attn_join_kernel(AttnTileArgs p, int parts) {
+    const int row = blockIdx.x / AH, h = blockIdx.x % AH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ __align__(16) float part_o[JOIN_WARPS][AHD];
+    __shared__ float part_l[JOIN_WARPS];
+    const bool mine = run_of_row(p, row) >= 0;
     const size_t g = (size_t)row * AH + h;
+    float gv[8];
+    if (warp == 0 && p.gate) get8(static_cast<const T *>(p.gate) + g * AHD + lane * 8, gv);
+    pdl_wait();
+    if (!mine) return;
     const float2 *ml = static_cast<const float2 *>(p.ws) + g * parts;
     const float *acc = reinterpret_cast<const float *>(static_cast<const float2 *>(p.ws) + (size_t)p.n_row * AH * parts) +
                        g * parts * AHD + lane * 8;
@@ -920,34 +968,46 @@ __global__ void __launch_bounds__(AH * 32) attn_join_kernel(AttnTileArgs p, int 
     for (int i = lane; i < parts; i += 32) mx = fmaxf(mx, ml[i].x);
     mx = warp_max(mx);
     float l = 0.0f, o[8] = {};
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-        float w = 0.0f;
-        if (i0 + lane < parts) {
-            const float2 t = ml[i0 + lane];
-            w = t.x == -INFINITY ? 0.0f : ex2(t.x - mx);
-            l = fmaf(w, t.y, l);
-        }
-        const int n = min(32, parts - i0);
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            float4 a = make_float4(0, 0, 0, 0), b = a;
-            if (wi != 0.0f) {  // (an empty part has no values)
-                a = *reinterpret_cast<const float4 *>(acc + (size_t)(i0 + i) * AHD);
-                b = *reinterpret_cast<const float4 *>(acc + (size_t)(i0 + i) * AHD + 4);
-            }
-            o[0] = fmaf(wi, a.x, o[0]); o[1] = fmaf(wi, a.y, o[1]); o[2] = fmaf(wi, a.z, o[2]); o[3] = fmaf(wi, a.w, o[3]);
-            o[4] = fmaf(wi, b.x, o[4]); o[5] = fmaf(wi, b.y, o[5]); o[6] = fmaf(wi, b.z, o[6]); o[7] = fmaf(wi, b.w, o[7]);
-        }
-    }
-    l = warp_sum(l);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    float gv[8];
-    if (p.gate) get8(static_cast<const T *>(p.gate) + g * AHD + lane * 8, gv);
+    constexpr int B = 8;
+    for (int i0 = warp; i0 < parts; i0 += JOIN_WARPS * B) {
+        float w[B], v[B][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        o[i] *= inv;
-        if (p.gate) o[i] *= sigmoid_f(gv[i]);
+        for (int k = 0; k < B; ++k) {
+            const int i = i0 + k * JOIN_WARPS;
+            w[k] = 0.0f;
+            if (i < parts) {
+                const float2 t = ml[i];
+                if (t.x != -INFINITY) {  // (an empty part has no values)
+                    w[k] = ex2(t.x - mx);
+                    l = fmaf(w[k], t.y, l);
+                    get8(acc + (size_t)i * AHD, v[k]);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < B; ++k)
+            if (w[k] != 0.0f) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = fmaf(w[k], v[k][e], o[e]);
+            }
+    }
+    put8(&part_o[warp][lane * 8], o);
+    if (lane == 0) part_l[warp] = l;
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < JOIN_WARPS; ++w) {
+        float t[8];
+        get8(&part_o[w][lane * 8], t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] += t[e];
+        l += part_l[w];
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        o[e] *= inv;
+        if (p.gate) o[e] *= sigmoid_fast(gv[e]);
     }
     put8(static_cast<T *>(p.out) + g * AHD + lane * 8, o);
 }
@@ -959,7 +1019,8 @@ TilePlan plan_for(int n_row, int n_run, int max_run, int max_len, int max_own, b
     TilePlan pl{};
     pl.pair = !shared && max_run > TM_TOK;
     const int toks = TM_TOK * (pl.pair ? 2 : 1), sms = kPlanSMs / (pl.pair ? 2 : 1);
-    pl.tiles = n_row / toks + (n_run < n_row ? n_run : n_row);
+    const int runs = n_run < n_row ? n_run : n_row;
+    pl.tiles = (n_row - runs) / toks + runs;  // the most that rows divided into so many runs can make
     if (!shared) {
         const long long most = (long long)n_run * ceil_div(max_run, toks);
         if (most < pl.tiles) pl.tiles = (int)most;
@@ -1028,8 +1089,18 @@ cudaError_t attn_tile_run(const AttnTileArgs &a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const int parts = pl.ns + pl.ns_own;
     if (parts > 1) {
-        (a.half ? attn_join_kernel<__half> : attn_join_kernel<float>)<<<a.n_row, AH * 32, 0, st>>>(a, parts);
-        e = cudaGetLastError();
+        // its launch, and the loads that do not depend on the parts, overlap the end of the kernel before
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)a.n_row * AH);
+        cfg.blockDim = dim3(JOIN_WARPS * 32);
+        cfg.stream = st;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = getenv("QW35_NO_PDL") ? 0 : 1;
+        e = a.half ? cudaLaunchKernelEx(&cfg, attn_join_kernel<__half>, a, parts)
+                   : cudaLaunchKernelEx(&cfg, attn_join_kernel<float>, a, parts);
     }
     return e;
 }

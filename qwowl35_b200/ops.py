@@ -7,6 +7,7 @@ stream.  There is no torch or CPU implementation behind any of them.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -146,27 +147,55 @@ def gqa_decode(q, gate, seq_len, max_len, chunk_ptrs, k_off, v_off, window=0, si
     return out
 
 
-def _ints(t, *shape):
+def _ints(t, dev, *shape):
     """A device int32 index array of the given shape."""
-    if t.dtype != torch.int32 or tuple(t.shape) != shape:
-        raise TypeError(f"int32 tensor of shape {shape} expected, got {t.dtype} {tuple(t.shape)}")
-    return _p(_dev(t))
+    if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise TypeError(f"contiguous int32 tensor of shape {shape} on cuda:{dev} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
-def _table(t):
+def _table(t, dev):
     """A device chunk table [rows, chunks] of 64-bit addresses."""
-    if t.dtype not in (torch.int64, torch.uint64) or t.dim() != 2:
-        raise TypeError("chunk_ptrs must be a 2-d tensor of 64-bit addresses")
-    return _p(_dev(t))
+    if t.dtype not in (torch.int64, torch.uint64) or t.dim() != 2 or t.get_device() != dev or not t.is_contiguous():
+        raise TypeError(f"chunk_ptrs must be a contiguous 2-d tensor of 64-bit addresses on cuda:{dev}")
+    return t.data_ptr()
 
 
-def _heads(t, n, dtype):
+def _heads(t, dev, n, dtype):
     """q, gate or out: [n, 16, 256] (or [n, 4096]) values of `dtype`; None passes."""
     if t is None:
         return None
-    if t.dtype != dtype or t.numel() != n * 4096:
-        raise TypeError(f"{dtype} tensor of {n} x 16 x 256 values expected, got {t.dtype} {tuple(t.shape)}")
-    return _p(_dev(t))
+    if t.dtype is not dtype or t.numel() != n * 4096 or t.get_device() != dev or not t.is_contiguous():
+        raise TypeError(f"contiguous {dtype} tensor of {n} x 16 x 256 values on cuda:{dev} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _head_dtype(dtype):
+    if dtype is torch.float32:
+        return 0
+    if dtype is torch.float16:
+        return 1
+    raise TypeError("q, gate and out must be float32 or float16")
+
+
+def _device_of(t):
+    if not t.is_cuda:
+        raise TypeError("device tensor expected")
+    return t.get_device()
+
+
+def _on_device(dev, name, *args):
+    """call() on device `dev` and its current stream (the raw handle: current_stream() costs 3 us a call)."""
+    if dev == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+
+
+@functools.lru_cache(maxsize=64)
+def _int32s(values):
+    return (C.c_int32 * len(values))(*values)
 
 
 def attn_append(qkv, q_norm_w, k_norm_w, rope_freq, rope_pos, sections, tok_seq, tok_pos, chunk_ptrs, k_off, v_off,
@@ -176,29 +205,24 @@ def attn_append(qkv, q_norm_w, k_norm_w, rope_freq, rope_pos, sections, tok_seq,
     qkv [n, >= 10240] f32 (rows may be strided); rope_pos [axes, n] int32 rotary positions, `sections` the pairs per
     axis; tok_seq / tok_pos [n] int32: chunk-table row (negative: padding, nothing written) and cache position.
     """
-    n = qkv.shape[0]
-    if qkv.dtype != torch.float32 or not qkv.is_cuda or qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] < 10240:
+    dev = _device_of(qkv)
+    if qkv.dtype is not torch.float32 or qkv.dim() != 2 or qkv.shape[1] < 10240 or qkv.stride(1) != 1:
         raise TypeError("qkv must be a float32 device tensor [n, >= 10240] with contiguous rows")
+    n, wide = qkv.shape
     for w, size in ((q_norm_w, 256), (k_norm_w, 256), (rope_freq, 32)):
-        if w.dtype != torch.float32 or w.numel() != size:
-            raise TypeError("norm weights (256) and rope_freq (32) must be float32")
-    q = torch.empty((n, 16, 256), dtype=dtype, device=qkv.device) if q is None else q
-    gate = torch.empty((n, 16, 256), dtype=dtype, device=qkv.device) if gate is None else gate
-    sec = (C.c_int32 * len(sections))(*sections)
-    call("qw35_cuda_attn_append", n, _p(qkv), qkv.stride(0) if n > 1 else qkv.shape[1], _p(_dev(q_norm_w)),
-         _p(_dev(k_norm_w)), _p(_dev(rope_freq)), _ints(rope_pos, len(sections), n), len(sections), sec,
-         1 if interleaved else 0, _ints(tok_seq, n), _ints(tok_pos, n), chunk_ptrs.shape[0], _table(chunk_ptrs),
-         chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0, _heads(q, n, dtype), _heads(gate, n, dtype),
-         _head_dtype(dtype), float(eps), _stream())
+        if w.dtype is not torch.float32 or w.numel() != size or w.get_device() != dev or not w.is_contiguous():
+            raise TypeError(f"norm weights (256) and rope_freq (32) must be contiguous float32 on cuda:{dev}")
+    half, axes = _head_dtype(dtype), len(sections)
+    if q is None:
+        q = qkv.new_empty((n, 16, 256), dtype=dtype)
+    if gate is None:
+        gate = torch.empty_like(q)
+    _on_device(dev, "qw35_cuda_attn_append", n, qkv.data_ptr(), qkv.stride(0) if n > 1 else wide, q_norm_w.data_ptr(),
+               k_norm_w.data_ptr(), rope_freq.data_ptr(), _ints(rope_pos, dev, axes, n), axes, _int32s(tuple(sections)),
+               1 if interleaved else 0, _ints(tok_seq, dev, n), _ints(tok_pos, dev, n), chunk_ptrs.shape[0],
+               _table(chunk_ptrs, dev), chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0, _heads(q, dev, n, dtype),
+               _heads(gate, dev, n, dtype), half, eps)
     return q, gate
-
-
-def _head_dtype(dtype):
-    if dtype == torch.float32:
-        return 0
-    if dtype == torch.float16:
-        return 1
-    raise TypeError("q, gate and out must be float32 or float16")
 
 
 def gqa_prefill_workspace(n_row: int, n_run: int, max_run: int, max_len: int, device="cuda"):
@@ -211,17 +235,21 @@ def gqa_prefill(q, gate, run_off, seq_len, max_run, max_len, chunk_ptrs, k_off, 
     """Causal attention of token runs over the cache that already holds them; [n, 4096] in q's type.
 
     run_off [runs + 1], seq_len [runs] int32: rows run_off[i]..run_off[i+1] of q are the last tokens of sequence i.
+    max_run, max_len: upper bounds of the runs' rows and of seq_len.
     """
+    dev, dtype = _device_of(q), q.dtype
     n, runs = q.shape[0], seq_len.numel()
     if chunk_ptrs.shape[0] < runs:
         raise ValueError("chunk_ptrs needs a row for every run")
+    half = _head_dtype(dtype)
     if out is None:
-        out = torch.empty((n, 4096), dtype=q.dtype, device=q.device)
+        out = q.new_empty((n, 4096))
     if ws is None:
-        ws = gqa_prefill_workspace(n, runs, max_run, max_len, q.device)
-    call("qw35_cuda_gqa_prefill", n, _heads(q, n, q.dtype), _heads(gate, n, q.dtype), _head_dtype(q.dtype), runs,
-         _ints(run_off, runs + 1), _ints(seq_len, runs), max_run, max_len, _table(chunk_ptrs), chunk_ptrs.shape[1],
-         k_off, v_off, 1 if kv_q8 else 0, window, sink, _heads(out, n, q.dtype), _p(ws), ws.numel(), _stream())
+        ws = q.new_empty(lib().qw35_cuda_gqa_prefill_workspace_bytes(n, runs, max_run, max_len), dtype=torch.uint8)
+    _on_device(dev, "qw35_cuda_gqa_prefill", n, _heads(q, dev, n, dtype), _heads(gate, dev, n, dtype), half, runs,
+               _ints(run_off, dev, runs + 1), _ints(seq_len, dev, runs), max_run, max_len, _table(chunk_ptrs, dev),
+               chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0, window, sink, _heads(out, dev, n, dtype),
+               _p(_dev(ws)), ws.numel())
     return out
 
 
@@ -237,15 +265,18 @@ def gqa_decode_shared(q, gate, seq_len, group_off, shared_len, max_shared, max_o
     group_off [groups + 1], shared_len [groups] int32: sequences group_off[g]..group_off[g+1] agree on their first
     shared_len[g] positions.  max_shared, max_own: upper bounds of shared_len and of seq_len - shared_len.
     """
+    dev, dtype = _device_of(q), q.dtype
     n, groups = q.shape[0], shared_len.numel()
     if chunk_ptrs.shape[0] < n:
         raise ValueError("chunk_ptrs needs a row for every sequence")
+    half = _head_dtype(dtype)
     if out is None:
-        out = torch.empty((n, 4096), dtype=q.dtype, device=q.device)
+        out = q.new_empty((n, 4096))
     if ws is None:
-        ws = gqa_decode_shared_workspace(n, groups, max_shared, max_own, q.device)
-    call("qw35_cuda_gqa_decode_shared", n, _heads(q, n, q.dtype), _heads(gate, n, q.dtype), _head_dtype(q.dtype),
-         _ints(seq_len, n), groups, _ints(group_off, groups + 1), _ints(shared_len, groups), max_shared, max_own,
-         _table(chunk_ptrs), chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0, window, sink,
-         _heads(out, n, q.dtype), _p(ws), ws.numel(), _stream())
+        ws = q.new_empty(lib().qw35_cuda_gqa_decode_shared_workspace_bytes(n, groups, max_shared, max_own),
+                         dtype=torch.uint8)
+    _on_device(dev, "qw35_cuda_gqa_decode_shared", n, _heads(q, dev, n, dtype), _heads(gate, dev, n, dtype), half,
+               _ints(seq_len, dev, n), groups, _ints(group_off, dev, groups + 1), _ints(shared_len, dev, groups),
+               max_shared, max_own, _table(chunk_ptrs, dev), chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0,
+               window, sink, _heads(out, dev, n, dtype), _p(_dev(ws)), ws.numel())
     return out
