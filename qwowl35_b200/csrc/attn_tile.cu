@@ -66,10 +66,10 @@ struct TileGeo {
     static constexpr bool LO_SMEM = HL && PAIR, LO_TMEM = HL && !PAIR;  // where Q's lo half is
     static constexpr uint32_t QB = LO_SMEM ? 2 * QBYTES : QBYTES;
     static constexpr int NST = LO_SMEM ? 3 : 5;          // stages: what 227 KB hold beside Q
-    // f16 planes: four warps issue the copies; q8_0: six convert, as many as fit 16 warps of 128 registers
-    static constexpr int LOADERS = Q8 ? 6 : 4;
+    // f16 planes: four warps issue the copies; q8_0: eight convert, each an eighth of a stage (at six, with two
+    // batches for some, a stage took 1.7 us and the products waited)
+    static constexpr int LOADERS = Q8 ? 8 : 4;
     static constexpr int THREADS = (SOFT_WARPS + LOADERS + 2) * 32;
-    enum : int { WSTEPS = STAGE / 512, STEPS = (WSTEPS + LOADERS - 1) / LOADERS };  // q8_0: passes over a stage, of a warp
     static constexpr int PARTS = HL && Q8 ? 2 : 1;       // stages of a tile: values, or their hi and lo halves
     static constexpr uint32_t RING = NST * STAGE, SMEM = QB + RING;
     static constexpr uint32_t S0 = 256;                  // TMEM columns: O, then the S buffers, then (LO_TMEM) Q's lo half
@@ -80,9 +80,10 @@ struct TileGeo {
 struct TilePlan {
     int pair;       // row tiles of two CTAs
     int tiles;      // row tiles (upper bound)
-    int ns;         // position splits of a row tile
+    int ns;         // position splits of a row tile (upper bound)
     int own_tiles;  // shared prefixes: sequences with a tail of their own, else 0
-    int ns_own;     // position splits of a tail
+    int ns_own;     // position splits of a tail (upper bound)
+    int each;       // kPlanTile tiles of a split
 };
 
 constexpr uint32_t kQlo = 384;  // TMEM columns of the lo half of Q
@@ -373,8 +374,9 @@ __device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan 
         s.part = tail ? pl.ns + split : split;
         s.lo = lo; s.hi_max = hi_max;
         s.a0 = a0; s.n1 = n1; s.t2 = t2;
-        s.begin = (int)((long long)total * split / ns);
-        s.end = (int)((long long)total * (split + 1) / ns);
+        const int each = pl.each * (kPlanTile / TK);
+        s.begin = min(total, split * each);
+        s.end = split == ns - 1 ? total : min(total, (split + 1) * each);
     }
     return nrow > 0;
 }
@@ -382,25 +384,30 @@ __device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan 
 __device__ __forceinline__ int tile_at(const TileShared &s, int i) { return i < s.n1 ? s.a0 + i : s.t2 + (i - s.n1); }
 
 // 8 codes of a q8_0 block (quarter j of the block at blk, 34 b bytes into its row) as they lie in memory: the
-// codes start 2 or 0 bytes past a 4-byte border by the block's parity, and only the words they touch are read
+// codes start 2 or 0 bytes past a 4-byte border by the block's parity, and only the words they touch are read.  An
+// even block's words hold its own d (first quarter) and the next block's (last quarter).
 struct Q8Raw {
     uint32_t w0, w1, w2;
-    unsigned short d;
 };
 __device__ __forceinline__ Q8Raw q8_fetch(const uint8_t *blk, int j, bool odd) {
     Q8Raw r;
     const uint32_t *w = reinterpret_cast<const uint32_t *>(blk + 2 + 8 * j - (odd ? 0 : 2));
-    r.d = *reinterpret_cast<const unsigned short *>(blk);
     r.w0 = w[0];
     r.w1 = w[1];
     r.w2 = odd ? 0u : w[2];
     return r;
 }
+// The block's d, by the whole warp; piece c of a row in lane c (or c and 16 + c, of two rows)
+__device__ __forceinline__ __half2 q8_scale(const Q8Raw &r, int c, bool odd) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t v = __shfl_sync(0xffffffffu, (c & 7) == 3 ? r.w2 : r.w0, odd ? (lane & ~3) - 1 : lane & ~3);
+    return __half2half2(__ushort_as_half((unsigned short)(odd ? v >> 16 : v)));
+}
 // d * code in f16: h rounded, l the remainder, exact (18 bits of product, 11 in h)
-__device__ __forceinline__ void q8_halves(const Q8Raw &r, bool odd, uint4 &h, uint4 &l) {
+__device__ __forceinline__ void q8_halves(const Q8Raw &r, __half2 d, bool odd, uint4 &h, uint4 &l) {
     const uint32_t sh = odd ? 0u : 16u;
     const uint32_t x[2] = {__funnelshift_r(r.w0, r.w1, sh) ^ 0x80808080u, __funnelshift_r(r.w1, r.w2, sh) ^ 0x80808080u};
-    const __half2 d = __half2half2(__ushort_as_half(r.d)), bias = __half2half2(__ushort_as_half((unsigned short)0x6480));
+    const __half2 bias = __half2half2(__ushort_as_half((unsigned short)0x6480));
     uint32_t hw[4], lw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // bytes of code + 128 in halves 1024 + byte; - 1152 is exact
@@ -482,35 +489,39 @@ struct Loader {
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&s.full[k])) : "memory");
     }
 
-    // q8_0 planes: a warp takes 32 pieces (a row of K, one or two of V) per step; the words of a stage are fetched
-    // while the one before it is converted
+    // q8_0 planes: a warp takes 8 rows of K, or 8 (of a pair, 16 half) rows of V, a piece a lane and row; the words of
+    // a stage are fetched while the one before it is converted
+    enum : int { Q8_ROWS = 8 };
     __device__ __forceinline__ int piece(bool v) const { return v ? rank * G::VP + (tid & 31) % G::VP : tid & 31; }
-    __device__ __forceinline__ int step_row(bool v, int step) const { return v ? step * G::CTAS + (tid & 31) / G::VP : step; }
+    __device__ __forceinline__ int first_row(bool v) const {
+        return (tid >> 5) * (v ? 8 * G::CTAS : 8) + (v && PAIR ? 8 * ((tid & 31) >> 4) : 0);
+    }
     __device__ __forceinline__ void fetch(const TileRef &h, Q8Raw *raw) const {
-        const int c = piece(h.v);
+        const int c = piece(h.v), r0 = first_row(h.v);
+        const bool odd = (c >> 2) & 1;
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(h.plane) + (size_t)(h.row0 + r0) * kKvQ8Row + 34 * (c >> 2);
+        const int a = lo - h.pos0 - r0, b = (h.plane ? hi : 0) - h.pos0 - r0;
+        if (a <= 0 && b >= Q8_ROWS) {
 #pragma unroll
-        for (int i = 0; i < G::STEPS; ++i) {
-            const int step = (tid >> 5) + i * G::LOADERS, r = step_row(h.v, step), pos = h.pos0 + r;
-            if (step < G::WSTEPS && pos >= lo && pos < hi && h.plane)
-                raw[i] = q8_fetch(reinterpret_cast<const uint8_t *>(h.plane) + (size_t)(h.row0 + r) * kKvQ8Row + 34 * (c >> 2), c & 3, (c >> 2) & 1);
-            else
-                raw[i] = Q8Raw{0u, 0u, 0u, 0};
+            for (int i = 0; i < Q8_ROWS; ++i) raw[i] = q8_fetch(src + i * kKvQ8Row, c & 3, odd);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Q8_ROWS; ++i) raw[i] = i >= a && i < b ? q8_fetch(src + i * kKvQ8Row, c & 3, odd) : Q8Raw{0u, 0u, 0u};
         }
     }
     __device__ __forceinline__ void convert(const TileRef &h, const Q8Raw *raw, int stage) {
-        const int c = piece(h.v), cs = h.v ? c - rank * G::VP : c;
-        const uint32_t blk = (uint32_t)(cs >> 3) * (h.v ? G::TK * 128u : G::KR * 128u);
+        const int c = piece(h.v), cs = h.v ? c - rank * G::VP : c, r0 = first_row(h.v);
+        const bool odd = (c >> 2) & 1;
+        // (r0 is a multiple of 8: row r0 + i of an atom column has its pieces at c ^ i)
+        const uint32_t at = (uint32_t)(cs >> 3) * (h.v ? G::TK * 128u : G::KR * 128u) + (uint32_t)(r0 >> 3) * 1024u + (uint32_t)(cs & 7) * 16u;
         const int k0 = acquire(stage * G::PARTS), k1 = HL ? acquire(stage * G::PARTS + 1) : 0;
-        const uint32_t d0 = ring + k0 * G::STAGE + blk, d1 = ring + k1 * G::STAGE + blk;
+        const uint32_t d0 = ring + k0 * G::STAGE + at, d1 = ring + k1 * G::STAGE + at;
 #pragma unroll
-        for (int i = 0; i < G::STEPS; ++i) {
-            const int step = (tid >> 5) + i * G::LOADERS, r = step_row(h.v, step);
-            if (step < G::WSTEPS) {
-                uint4 vh, vl;
-                q8_halves(raw[i], (c >> 2) & 1, vh, vl);
-                sts16(d0 + sw128_off(r, cs & 7), vh);
-                if constexpr (HL) sts16(d1 + sw128_off(r, cs & 7), vl);
-            }
+        for (int i = 0; i < Q8_ROWS; ++i) {
+            uint4 vh, vl;
+            q8_halves(raw[i], q8_scale(raw[i], c, odd), odd, vh, vl);
+            sts16((d0 ^ (i * 16u)) + i * 128u, vh);
+            if constexpr (HL) sts16((d1 ^ (i * 16u)) + i * 128u, vl);
         }
         mbar_arrive(&s.full[k0]);
         if constexpr (HL) mbar_arrive(&s.full[k1]);
@@ -519,24 +530,27 @@ struct Loader {
     __device__ __forceinline__ void run() {
         if (n <= 0) return;
         if constexpr (Q8) {
-            Q8Raw a[G::STEPS], b[G::STEPS];
-            TileRef ha = ref(0), hb;
+            // (tile addresses come from memory, too: one stage further ahead)
+            Q8Raw a[Q8_ROWS], b[Q8_ROWS];
+            TileRef ha = ref(0), hb = ref(1);
             fetch(ha, a);
             for (int i = 0; i < 2 * n; i += 2) {
-                hb = ref(i + 1);
                 fetch(hb, b);
+                const TileRef hc = ref(min(i + 2, 2 * n - 1));
                 convert(ha, a, i);
-                if (i + 2 < 2 * n) {
-                    ha = ref(i + 2);
-                    fetch(ha, a);
-                }
+                if (i + 2 < 2 * n) fetch(hc, a);
+                const TileRef hd = ref(min(i + 3, 2 * n - 1));
                 convert(hb, b, i + 1);
+                ha = hc;
+                hb = hd;
             }
         } else {
+            TileRef h = ref(0);
             for (int i = 0; i < 2 * n; ++i) {
-                const TileRef h = ref(i);
+                const TileRef next = ref(min(i + 1, 2 * n - 1));  // (its chunk address comes from memory)
                 if (h.v) copy<true>(h, i);
                 else copy<false>(h, i);
+                h = next;
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
@@ -686,6 +700,13 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
     }
     pdl_trigger();
     if (!__syncthreads_or(work)) return;
+    if (s.begin == s.end && pl.ns + pl.ns_own > 1) {  // (both CTAs of a pair) nothing to attend in this part
+        if (tid < s.nrow * AGRP) {
+            const size_t g = (size_t)(s.row0 + tid / AGRP) * AH + s.kvh * AGRP + tid % AGRP;
+            static_cast<float2 *>(p.ws)[g * (pl.ns + pl.ns_own) + s.part] = make_float2(-INFINITY, 0.0f);
+        }
+        return;
+    }
     if (warp == MMA_WARP) tmem_take<PAIR>(&s.tmem);
     tc_fence_before();
     if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist
@@ -1027,15 +1048,19 @@ TilePlan plan_for(int n_row, int n_run, int max_run, int max_len, int max_own, b
         const int units = pl.tiles * AKV, kv = ceil_div(max_len, kPlanTile);
         pl.ns = units >= sms ? 1 : sms / units;
         if (pl.ns > kv) pl.ns = kv;
+        pl.each = ceil_div(kv, pl.ns);
+        pl.ns = ceil_div(kv, pl.each);
         return pl;
     }
-    // shared prefixes: parts of equal length, one wave of CTAs at most for the prefixes
+    // Shared prefixes.  Parts of one length: what one wave of CTAs would get each, a tail counting as its setup (a
+    // tile's time) and half the longest.  Several groups may be much shorter than the longest, by which the host has
+    // to plan, and leave SMs without a part: half the length then, two waves at most.
     const int kv = ceil_div(max_len, kPlanTile), kv_own = ceil_div(max_own, kPlanTile) + 1;
-    const long long work = (long long)AKV * ((long long)pl.tiles * kv + (long long)n_row * kv_own);
-    const int each = ceil_div(work, kPlanSMs);
-    pl.ns = kv > 0 ? ceil_div(kv, each) : 1;
+    const long long work = (long long)AKV * ((long long)pl.tiles * kv + (long long)n_row * (1 + kv_own / 2));
+    pl.each = ceil_div(work, (n_run > 1 ? 2 : 1) * kPlanSMs);
+    pl.ns = kv > 0 ? ceil_div(kv, pl.each) : 1;
     pl.own_tiles = n_row;
-    pl.ns_own = ceil_div(kv_own, each);
+    pl.ns_own = ceil_div(kv_own, pl.each);
     return pl;
 }
 
