@@ -57,7 +57,8 @@ int qw35_cuda_set_device(int device, char *err, uintptr_t err_len) {
 }
 
 uint32_t qw35_cuda_device_error(void) {
-    return qw35::device_error_read_and_clear() | qw35::attn_tile_error_read_and_clear();
+    return qw35::device_error_read_and_clear() | qw35::attn_append_error_read_and_clear() |
+           qw35::attn_tile_error_read_and_clear();
 }
 
 const char *qw35_cuda_build_info(void) { return "qw35cuda sm_100a (" __DATE__ ")"; }

@@ -175,6 +175,7 @@ struct AttnTileArgs {
 size_t attn_tile_workspace_bytes(int n_row, int n_run, int max_run, int max_len, int max_own);
 cudaError_t attn_tile_run(const AttnTileArgs &a, cudaStream_t st);
 
+unsigned int attn_append_error_read_and_clear();
 unsigned int attn_tile_error_read_and_clear();
 unsigned int device_error_read_and_clear();
 

@@ -11,7 +11,7 @@ import functools
 
 import torch
 
-from ._lib import call, lib
+from ._lib import call, check, err_buf, lib
 
 GF4, Q8_0, Q4_K, Q5_K, Q6_K = 100, 8, 12, 13, 14
 EXACT = 1
@@ -154,6 +154,13 @@ def _ints(t, dev, *shape):
     return t.data_ptr()
 
 
+def _floats(t, dev, size):
+    """A device float32 vector of the given size (norm weights, frequencies)."""
+    if t.dtype is not torch.float32 or t.numel() != size or t.get_device() != dev or not t.is_contiguous():
+        raise TypeError(f"contiguous float32 tensor of {size} values on cuda:{dev} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
 def _table(t, dev):
     """A device chunk table [rows, chunks] of 64-bit addresses."""
     if t.dtype not in (torch.int64, torch.uint64) or t.dim() != 2 or t.get_device() != dev or not t.is_contiguous():
@@ -185,9 +192,10 @@ def _device_of(t):
 
 
 def _on_device(dev, name, *args):
-    """call() on device `dev` and its current stream (the raw handle: current_stream() costs 3 us a call)."""
+    """call() on device `dev` and its current stream (by its raw handle: current_stream() costs 3 us a call)."""
     if dev == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+        e = err_buf()
+        check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev), e, 1024), e)
     else:
         with torch.cuda.device(dev):
             call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
@@ -209,16 +217,13 @@ def attn_append(qkv, q_norm_w, k_norm_w, rope_freq, rope_pos, sections, tok_seq,
     if qkv.dtype is not torch.float32 or qkv.dim() != 2 or qkv.shape[1] < 10240 or qkv.stride(1) != 1:
         raise TypeError("qkv must be a float32 device tensor [n, >= 10240] with contiguous rows")
     n, wide = qkv.shape
-    for w, size in ((q_norm_w, 256), (k_norm_w, 256), (rope_freq, 32)):
-        if w.dtype is not torch.float32 or w.numel() != size or w.get_device() != dev or not w.is_contiguous():
-            raise TypeError(f"norm weights (256) and rope_freq (32) must be contiguous float32 on cuda:{dev}")
     half, axes = _head_dtype(dtype), len(sections)
     if q is None:
         q = qkv.new_empty((n, 16, 256), dtype=dtype)
     if gate is None:
         gate = torch.empty_like(q)
-    _on_device(dev, "qw35_cuda_attn_append", n, qkv.data_ptr(), qkv.stride(0) if n > 1 else wide, q_norm_w.data_ptr(),
-               k_norm_w.data_ptr(), rope_freq.data_ptr(), _ints(rope_pos, dev, axes, n), axes, _int32s(tuple(sections)),
+    _on_device(dev, "qw35_cuda_attn_append", n, qkv.data_ptr(), qkv.stride(0) if n > 1 else wide,
+               _floats(q_norm_w, dev, 256), _floats(k_norm_w, dev, 256), _floats(rope_freq, dev, 32), _ints(rope_pos, dev, axes, n), axes, _int32s(tuple(sections)),
                1 if interleaved else 0, _ints(tok_seq, dev, n), _ints(tok_pos, dev, n), chunk_ptrs.shape[0],
                _table(chunk_ptrs, dev), chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0, _heads(q, dev, n, dtype),
                _heads(gate, dev, n, dtype), half, eps)

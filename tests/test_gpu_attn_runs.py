@@ -227,6 +227,46 @@ def test_append_matches_the_formulas(half, q8, sections, interleaved):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("half,q8", [(False, False), (True, False), (True, True)])
+@pytest.mark.parametrize("n,off", [(148, 0), (591, 0), (1500, 0), (1500, 1)])
+def test_append_of_many_tokens(half, q8, n, off):
+    """One to eleven tokens an SM, a padding token among every 37; off: rows that no 16-byte copy can fetch."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    c = Cache([n], q8, 3)
+    g = torch.Generator("cuda").manual_seed(n + off)
+    qkv = torch.randn(n, 10240 + 8, device="cuda", generator=g)[:, off:10240 + off]
+    qw, kw = (1 + 0.2 * torch.randn(256, device="cuda", generator=g) for _ in range(2))
+    pos = torch.randint(0, 262144, (3, n), generator=torch.Generator().manual_seed(n)).int().cuda()
+    t = torch.arange(n, device="cuda")
+    pad = t % 37 == 5
+    seq = torch.where(pad, -1, 0).int()
+    at = ((t * 7919) % n).int()
+    q0 = torch.full((n, H, D), 7.0, dtype=kind, device="cuda")
+    before = c.rows().clone()
+    q, gate = ops.attn_append(qkv, qw, kw, FREQ.cuda(), pos, (11, 11, 10), seq, at, c.ptrs(), c.k_off, c.v_off, eps=EPS, dtype=kind,
+                              kv_q8=q8, q=q0, gate=q0.clone())
+    rq, rg, rk, rv = append_reference(qkv, qw, kw, FREQ.cuda(), pos, axes_of((11, 11, 10), True))
+    near(q[~pad], rq[~pad], kind, rq.abs().amax(-1, keepdim=True)[~pad])
+    assert torch.equal(gate[~pad], rg[~pad].to(kind))
+    assert bool((q[pad] == 7).all()) and bool((gate[pad] == 7).all())
+    chunk, p = c.ids[0].cuda()[at.long() // CH], at.long() % CH
+    k, v = c.rows()[chunk, 0, :, p], c.rows()[chunk, 1, :, p]
+    old = before[chunk, :, :, p]
+    assert torch.equal(torch.stack([k, v], 1)[pad].view(torch.uint8), old[pad].view(torch.uint8))
+    if q8:
+        for got, ref in ((k, rk), (v, rv)):
+            blocks = ref.view(n, KV, 8, 32)[~pad]
+            d = blocks.abs().amax(-1, keepdim=True) / 127
+            value = (got[..., 2:].view(torch.int8).double() * got[..., :2].view(torch.float16).double())[~pad]
+            assert bool(((value - blocks).abs() <= d * (0.5 + 127 * 2.0 ** -11 + 0.01)).all())
+    else:
+        near(k[~pad], rk[~pad], torch.float16, rk.abs().amax(-1, keepdim=True)[~pad])
+        assert torch.equal(v[~pad], rv[~pad].half())
+    assert _lib.lib().qw35_cuda_device_error() == 0
+
+
+@pytest.mark.gpu
 def test_append_agrees_with_the_single_token_preprocess():
     """One axis and near positions (where the f32 angle is exact enough): the same cache rows, q and gate."""
     from qwowl35_b200 import ops
