@@ -69,7 +69,13 @@ struct TileGeo {
     // f16 planes: four warps issue the copies; q8_0: eight convert, each an eighth of a stage (at six, with two
     // batches for some, a stage took 1.7 us and the products waited)
     static constexpr int LOADERS = Q8 ? 8 : 4;
-    static constexpr int THREADS = (SOFT_WARPS + LOADERS + 2) * 32;
+    // f16 over q8_0: 18 warps leave 96 registers a thread and softmax needs more (8192-token prompt 594 us with the
+    // split, 657 without); f32's smaller tiles do not, and the 14 warps over f16 planes have 128 (449 us; split 463)
+    static constexpr bool SPLIT = Q8 && !HL;
+    static constexpr int THREADS = (SOFT_WARPS + LOADERS + (SPLIT ? 4 : 2)) * 32;  // and products, relay (two idle: whole groups of four)
+    // registers a thread of softmax warps, loaders and the last four warps, within the launch's 96 a thread
+    static constexpr int SOFT_REGS = 136, LOAD_REGS = 80, REST_REGS = 48;
+    static_assert(!SPLIT || SOFT_WARPS * SOFT_REGS + LOADERS * LOAD_REGS + 4 * REST_REGS <= THREADS / 32 * 96, "registers");
     static constexpr int PARTS = HL && Q8 ? 2 : 1;       // stages of a tile: values, or their hi and lo halves
     static constexpr uint32_t RING = NST * STAGE, SMEM = QB + RING;
     static constexpr uint32_t S0 = 256;                  // TMEM columns: O, then the S buffers, then (LO_TMEM) Q's lo half
@@ -99,6 +105,13 @@ struct __align__(16) TileShared {
     int hi[TM_TOK], sk[TM_TOK], rs[TM_TOK];
     float ex[2][2][TM_ROWS];           // row maxima (then sums) exchanged between the two column halves
 };
+
+template <bool SPLIT, int REGS, bool MORE>
+__device__ __forceinline__ void set_regs() {
+    if constexpr (!SPLIT) return;
+    else if constexpr (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
 
 // ---- two CTAs ---------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cta_rank() {
@@ -186,13 +199,16 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t *bar, uint32_t parity)
     return ok != 0;
 }
 __device__ __forceinline__ void tw(uint64_t *bar, uint32_t parity, TileShared &s, unsigned code) {
-    if (*(volatile int *)&s.abort || try_wait_cluster(bar, parity)) return;
-    const unsigned long long t0 = globaltimer();
-    while (!try_wait_cluster(bar, parity)) {
-        if (globaltimer() - t0 > kTimeoutNs) {
+    if (try_wait_cluster(bar, parity)) return;
+    unsigned long long t0 = 0;
+    while (!*(volatile int *)&s.abort) {
+        for (int i = 0; i < 16; ++i)  // (a look at the clock costs more than one at the barrier)
+            if (try_wait_cluster(bar, parity)) return;
+        const unsigned long long t = globaltimer();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kTimeoutNs) {
             atomicOr(&g_dev_error, code);
             *(volatile int *)&s.abort = 1;
-            return;
         }
     }
 }
@@ -715,18 +731,20 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
     const uint32_t tmem = s.tmem;
 
     if (warp >= SOFT_WARPS && warp < MMA_WARP) {
+        set_regs<G::SPLIT, G::LOAD_REGS, false>();
         Loader<HL, Q8, PAIR> ld{p, s, sbase + G::QB, tid - SOFT_WARPS * 32, rank, s.lo, s.hi_max, s.end - s.begin};
         ld.run();
-    } else if (warp == MMA_WARP) {
-        if (rank == 0) {
+    } else if (warp >= MMA_WARP) {
+        set_regs<G::SPLIT, G::REST_REGS, false>();
+        if (warp == MMA_WARP && rank == 0) {
             Products<HL, Q8, PAIR> mm{s, sbase, sbase + G::QB, tmem};
             mm.run();
+        } else if (warp == MMA_WARP + 1 && lane == 0) {
+            relay<HL, Q8, PAIR>(s, rank);
         }
         __syncwarp();
-    } else if (warp == MMA_WARP + 1) {
-        if (lane == 0) relay<HL, Q8, PAIR>(s, rank);
-        __syncwarp();
     } else {
+        set_regs<G::SPLIT, G::SOFT_REGS, true>();
         // softmax warps: row = TMEM lane; two groups of four, each a half of the columns (positions, then dims).
         // (Groups that take whole tiles in turn overlap better with each other, but each then holds an S buffer
         // twice as long, and with two buffers that is what the products wait for: 2.0 us a tile against 1.3.)
