@@ -157,7 +157,10 @@ int qw35_cuda_gqa_decode_noalloc(uint32_t n_seq, const float *q, const float *ga
 // kv_cache_type).  dtype: 0 f32, 1 f16, of q, gate and out.  All index arrays are
 // device memory, so the calls can be captured into a CUDA graph and replayed
 // over other lengths within the host's upper bounds.  q, gate and out are
-// [rows][16][256], 16-byte aligned, as is every chunk address.
+// [rows][16][256], 16-byte aligned, as is every chunk address; an f32 q and what
+// the cache stands for lie within the f16 range.  A workspace serves one call at
+// a time: calls that may overlap on the GPU (other streams, other graphs) need
+// their own.
 
 // Appends n_tok tokens to the cache: per-head RMS norm of q and k, rotary
 // positions on dims [0, 64) (NeoX pairs i, i + 32), K and V rows written for table
@@ -182,8 +185,8 @@ int qw35_cuda_attn_append(uint32_t n_tok, const float *qkv, uint32_t qkv_stride,
 // seq_len[i]; the run's row t attends positions [0, seq_len[i] - run length + t],
 // cut by window and sink as in qw35_cuda_gqa_decode.  n_row is the number of rows
 // of q; rows outside every run are left as they were.  max_run and max_len are
-// upper bounds of a run's rows and of seq_len.  Cache rows within seq_len[i] have
-// to be finite; what lies behind them is not looked at.
+// upper bounds of a run's rows and of seq_len.  The cache rows of [0, seq_len[i])
+// have to be finite, masked or not; what lies behind them is not looked at.
 uint64_t qw35_cuda_gqa_prefill_workspace_bytes(uint32_t n_row, uint32_t n_run, uint32_t max_run, uint32_t max_len);
 int qw35_cuda_gqa_prefill(uint32_t n_row, const void *q, const void *gate, uint32_t dtype, uint32_t n_run,
                           const int32_t *run_off, const int32_t *seq_len, uint32_t max_run, uint32_t max_len,
@@ -195,8 +198,10 @@ int qw35_cuda_gqa_prefill(uint32_t n_row, const void *q, const void *gate, uint3
 // computes for them, with each prefix read once per group.  Sequences
 // [group_off[g], group_off[g+1]) have the same keys and values at positions
 // [0, shared_len[g]) (read through the group's first table row); the rest of
-// their seq_len[i] positions are their own.  max_shared and max_own are upper
-// bounds of shared_len and of seq_len[i] - shared_len[g].
+// their seq_len[i] positions are their own.  A sequence may end inside the
+// prefix.  Sequences of no group are left as they were.  max_shared and max_own
+// are upper bounds of shared_len and of seq_len[i] - shared_len[g].  The cache
+// rows in reach have to be finite, as above.
 uint64_t qw35_cuda_gqa_decode_shared_workspace_bytes(uint32_t n_seq, uint32_t n_group, uint32_t max_shared,
                                                      uint32_t max_own);
 int qw35_cuda_gqa_decode_shared(uint32_t n_seq, const void *q, const void *gate, uint32_t dtype,

@@ -338,7 +338,7 @@ __device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan 
         }
     }
     const int row0 = w.row0;
-    if (row0 < 0 || row0 + nrow > p.n_row) nrow = 0;
+    if (w.begin < 0 || row0 < 0 || row0 + nrow > p.n_row) nrow = 0;  // (offsets that make no sense)
     // lane = token of the CTA's tile; a pair walks the positions that either of its tiles needs
     int lo = 0, hi_max = 0, rs_min = 0x7fffffff, sk_max = 0;
     for (int e = 0; e < CTAS; ++e) {
@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
         s.abort = 0;
         fence_barrier_init();
     }
-    pdl_trigger();
+    if (pl.ns + pl.ns_own > 1) pdl_trigger();  // (the join comes next)
     if (!__syncthreads_or(work)) return;
     if (s.begin == s.end && pl.ns + pl.ns_own > 1) {  // (both CTAs of a pair) nothing to attend in this part
         if (tid < s.nrow * AGRP) {

@@ -454,6 +454,94 @@ def test_shared_agrees_with_gqa_decode():
     check_rows(out, ref, False, False)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+def test_shared_leaves_sequences_of_no_group(half):
+    """Sequences before the first group, between groups and behind the last keep what out held."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    cache = Cache([300] * 8, False, 2).fill([300] * 8, 3)
+    q, gt = some(8, 1, kind), some(8, 2, kind)
+    out = torch.full((8, H * D), 5.0, dtype=kind, device="cuda")
+    ops.gqa_decode_shared(q, gt, ints(*[280] * 8), ints(1, 1, 3), ints(64, 128), 128, 216, cache.ptrs(), cache.k_off, cache.v_off,
+                          out=out)
+    # (groups [1, 1) and [1, 3); the second reads its 128 shared positions through table row 1)
+    assert bool((out[0] == 5).all()) and bool((out[3:] == 5).all())
+    ref = []
+    for i in (1, 2):
+        (k, v), (k1, v1) = cache.sequence(i, 280), cache.sequence(1, 280)
+        k, v = torch.cat([k1[:, :128], k[:, 128:]], 1), torch.cat([v1[:, :128], v[:, 128:]], 1)
+        ref.append((i, *attend(q[i], gt[i], k, v, 280), 280))
+    check_rows(out, ref, half, False)
+
+
+@pytest.mark.gpu
+def test_bounds_below_the_lengths_still_attend_everything():
+    """max_len, max_shared and max_own size the split, not the work."""
+    from qwowl35_b200 import ops
+    cache = Cache([3000, 3000], False, 2).fill([3000, 3000], 3)
+    q, gt = some(20, 1, torch.float32), some(20, 2, torch.float32)
+    out = ops.gqa_prefill(q, gt, ints(0, 20), ints(3000), 20, 200, cache.ptrs()[:1].contiguous(), cache.k_off, cache.v_off)
+    k, v = cache.sequence(0, 3000)
+    check_rows(out, [(r, *attend(q[r], gt[r], k, v, 2981 + r), 2981 + r) for r in (0, 7, 19)], False, False)
+    cache.ids[1, :8] = cache.ids[0, :8]
+    out = ops.gqa_decode_shared(q[:2], gt[:2], ints(3000, 2900), ints(0, 2), ints(2048), 100, 50, cache.ptrs(), cache.k_off,
+                                cache.v_off)
+    ref = []
+    for i, n in enumerate((3000, 2900)):
+        k, v = cache.sequence(i, n)
+        ref.append((i, *attend(q[i], gt[i], k, v, n), n))
+    check_rows(out, ref, False, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("off,lens", [((-64, 32), (500,)), ((0, 90), (500,)), ((20, 10, 40), (500, 500)), ((0, 40), (-7,)), ((0, 0), (9,))])
+def test_offsets_that_make_no_sense_are_skipped(off, lens):
+    """Runs outside the rows, backwards or empty, and lengths below zero: nothing is read or written out of range."""
+    from qwowl35_b200 import ops
+    cache = Cache([512] * len(lens), False, 2).fill([512] * len(lens), 3)
+    q = some(40, 1, torch.float16)
+    for gate in (None, q):
+        out = ops.gqa_prefill(q, gate, ints(*off), ints(*lens), 40, 512, cache.ptrs(), cache.k_off, cache.v_off)
+    tables = cache.ptrs()[[0] * 40].contiguous()
+    ops.gqa_decode_shared(q, q, ints(*[500] * 40), ints(*off), ints(*lens), 500, 100, tables, cache.k_off, cache.v_off, out=out)
+    torch.cuda.synchronize()
+    assert _lib.lib().qw35_cuda_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_more_runs_than_a_warp_and_one_row_each():
+    """70 single-token runs and 45 groups: the searches go beyond one warp's width."""
+    from qwowl35_b200 import ops
+    lens = [1 + (i * 29) % 300 for i in range(70)]
+    cache = Cache(lens, True, 2).fill(lens, 3)
+    q, gt = some(70, 1, torch.float32), some(70, 2, torch.float32)
+    table = cache.ptrs()
+    out = ops.gqa_prefill(q, gt, ints(*range(71)), ints(*lens), 1, max(lens), table, cache.k_off, cache.v_off, kv_q8=True)
+    ref = []
+    for i, n in enumerate(lens):
+        k, v = cache.sequence(i, n)
+        ref.append((i, *attend(q[i], gt[i], k, v, n), n))
+    check_rows(out, ref, False, True)
+    out = ops.gqa_decode_shared(q, gt, ints(*lens), ints(*range(71)), ints(*[n // 2 for n in lens]), 150, 151, table, cache.k_off,
+                                cache.v_off, kv_q8=True)
+    check_rows(out, ref, False, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+def test_out_may_be_the_gate(half):
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    cache = Cache([700], False, 2).fill([700], 3)
+    for rows in (5, 700):
+        q, gt = some(rows, 1, kind), some(rows, 2, kind)
+        args = (ints(0, rows), ints(700), rows, 700, cache.ptrs(), cache.k_off, cache.v_off)
+        want = ops.gqa_prefill(q, gt, *args)
+        got = ops.gqa_prefill(q, gt, *args, out=gt)
+        assert torch.equal(got.view(want.shape), want)
+
+
 # ---- together, captured, on several streams ---------------------------------------------------
 
 @pytest.mark.gpu
