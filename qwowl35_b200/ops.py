@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import threading
 
 import torch
 
@@ -147,7 +148,10 @@ def gqa_decode(q, gate, seq_len, max_len, chunk_ptrs, k_off, v_off, window=0, si
     return out
 
 
-def _ints(t, dev, *shape):
+# The calls below check their tensors on every call, so each check is a few attribute reads and nothing more: at a
+# single token the wrapper is most of what a call costs (16 us of host time, 4 us on the GPU).
+
+def _ints(t, dev, shape):
     """A device int32 index array of the given shape."""
     if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
         raise TypeError(f"contiguous int32 tensor of shape {shape} on cuda:{dev} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -191,14 +195,22 @@ def _device_of(t):
     return t.get_device()
 
 
-def _on_device(dev, name, *args):
-    """call() on device `dev` and its current stream (by its raw handle: current_stream() costs 3 us a call)."""
-    if dev == torch._C._cuda_getDevice():
-        e = err_buf()
-        check(getattr(lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev), e, 1024), e)
-    else:
+class _Errors(threading.local):
+    def __init__(self):
+        self.buf = err_buf()
+
+
+_errors = _Errors()
+
+
+def _on_device(dev, func, *args):
+    """call() of an entry point on device `dev` and its current stream (by its raw handle: current_stream() costs 3 us)."""
+    if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
-            call(name, *args, torch._C._cuda_getCurrentRawStream(dev))
+            return _on_device(dev, func, *args)
+    e = _errors.buf
+    if not func(*args, torch._C._cuda_getCurrentRawStream(dev), e, 1024):
+        check(0, e)
 
 
 @functools.lru_cache(maxsize=64)
@@ -214,19 +226,26 @@ def attn_append(qkv, q_norm_w, k_norm_w, rope_freq, rope_pos, sections, tok_seq,
     axis; tok_seq / tok_pos [n] int32: chunk-table row (negative: padding, nothing written) and cache position.
     """
     dev = _device_of(qkv)
-    if qkv.dtype is not torch.float32 or qkv.dim() != 2 or qkv.shape[1] < 10240 or qkv.stride(1) != 1:
+    shape = qkv.shape
+    if qkv.dtype is not torch.float32 or len(shape) != 2 or shape[1] < 10240 or qkv.stride(1) != 1:
         raise TypeError("qkv must be a float32 device tensor [n, >= 10240] with contiguous rows")
-    n, wide = qkv.shape
-    half, axes = _head_dtype(dtype), len(sections)
+    n, axes, half = shape[0], len(sections), _head_dtype(dtype)
     if q is None:
         q = qkv.new_empty((n, 16, 256), dtype=dtype)
+        q_ptr = q.data_ptr()
+    else:
+        q_ptr = _heads(q, dev, n, dtype)
     if gate is None:
         gate = torch.empty_like(q)
-    _on_device(dev, "qw35_cuda_attn_append", n, qkv.data_ptr(), qkv.stride(0) if n > 1 else wide,
-               _floats(q_norm_w, dev, 256), _floats(k_norm_w, dev, 256), _floats(rope_freq, dev, 32), _ints(rope_pos, dev, axes, n), axes, _int32s(tuple(sections)),
-               1 if interleaved else 0, _ints(tok_seq, dev, n), _ints(tok_pos, dev, n), chunk_ptrs.shape[0],
-               _table(chunk_ptrs, dev), chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0, _heads(q, dev, n, dtype),
-               _heads(gate, dev, n, dtype), half, eps)
+        gate_ptr = gate.data_ptr()
+    else:
+        gate_ptr = _heads(gate, dev, n, dtype)
+    table = chunk_ptrs.shape
+    _on_device(dev, lib().qw35_cuda_attn_append, n, qkv.data_ptr(), qkv.stride(0) if n > 1 else shape[1],
+               _floats(q_norm_w, dev, 256), _floats(k_norm_w, dev, 256), _floats(rope_freq, dev, 32),
+               _ints(rope_pos, dev, (axes, n)), axes, _int32s(tuple(sections)), 1 if interleaved else 0,
+               _ints(tok_seq, dev, (n,)), _ints(tok_pos, dev, (n,)), table[0], _table(chunk_ptrs, dev), table[1], k_off,
+               v_off, 1 if kv_q8 else 0, q_ptr, gate_ptr, half, eps)
     return q, gate
 
 
@@ -243,18 +262,20 @@ def gqa_prefill(q, gate, run_off, seq_len, max_run, max_len, chunk_ptrs, k_off, 
     max_run, max_len: upper bounds of the runs' rows and of seq_len.
     """
     dev, dtype = _device_of(q), q.dtype
-    n, runs = q.shape[0], seq_len.numel()
-    if chunk_ptrs.shape[0] < runs:
+    n, runs, table = q.shape[0], seq_len.numel(), chunk_ptrs.shape
+    if table[0] < runs:
         raise ValueError("chunk_ptrs needs a row for every run")
-    half = _head_dtype(dtype)
+    half, L = _head_dtype(dtype), lib()
     if out is None:
         out = q.new_empty((n, 4096))
+        out_ptr = out.data_ptr()
+    else:
+        out_ptr = _heads(out, dev, n, dtype)
     if ws is None:
-        ws = q.new_empty(lib().qw35_cuda_gqa_prefill_workspace_bytes(n, runs, max_run, max_len), dtype=torch.uint8)
-    _on_device(dev, "qw35_cuda_gqa_prefill", n, _heads(q, dev, n, dtype), _heads(gate, dev, n, dtype), half, runs,
-               _ints(run_off, dev, runs + 1), _ints(seq_len, dev, runs), max_run, max_len, _table(chunk_ptrs, dev),
-               chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0, window, sink, _heads(out, dev, n, dtype),
-               _p(_dev(ws)), ws.numel())
+        ws = q.new_empty(L.qw35_cuda_gqa_prefill_workspace_bytes(n, runs, max_run, max_len), dtype=torch.uint8)
+    _on_device(dev, L.qw35_cuda_gqa_prefill, n, _heads(q, dev, n, dtype), _heads(gate, dev, n, dtype), half, runs,
+               _ints(run_off, dev, (runs + 1,)), _ints(seq_len, dev, (runs,)), max_run, max_len, _table(chunk_ptrs, dev),
+               table[1], k_off, v_off, 1 if kv_q8 else 0, window, sink, out_ptr, _p(_dev(ws)), ws.numel())
     return out
 
 
@@ -271,17 +292,19 @@ def gqa_decode_shared(q, gate, seq_len, group_off, shared_len, max_shared, max_o
     shared_len[g] positions.  max_shared, max_own: upper bounds of shared_len and of seq_len - shared_len.
     """
     dev, dtype = _device_of(q), q.dtype
-    n, groups = q.shape[0], shared_len.numel()
-    if chunk_ptrs.shape[0] < n:
+    n, groups, table = q.shape[0], shared_len.numel(), chunk_ptrs.shape
+    if table[0] < n:
         raise ValueError("chunk_ptrs needs a row for every sequence")
-    half = _head_dtype(dtype)
+    half, L = _head_dtype(dtype), lib()
     if out is None:
         out = q.new_empty((n, 4096))
+        out_ptr = out.data_ptr()
+    else:
+        out_ptr = _heads(out, dev, n, dtype)
     if ws is None:
-        ws = q.new_empty(lib().qw35_cuda_gqa_decode_shared_workspace_bytes(n, groups, max_shared, max_own),
-                         dtype=torch.uint8)
-    _on_device(dev, "qw35_cuda_gqa_decode_shared", n, _heads(q, dev, n, dtype), _heads(gate, dev, n, dtype), half,
-               _ints(seq_len, dev, n), groups, _ints(group_off, dev, groups + 1), _ints(shared_len, dev, groups),
-               max_shared, max_own, _table(chunk_ptrs, dev), chunk_ptrs.shape[1], k_off, v_off, 1 if kv_q8 else 0,
-               window, sink, _heads(out, dev, n, dtype), _p(_dev(ws)), ws.numel())
+        ws = q.new_empty(L.qw35_cuda_gqa_decode_shared_workspace_bytes(n, groups, max_shared, max_own), dtype=torch.uint8)
+    _on_device(dev, L.qw35_cuda_gqa_decode_shared, n, _heads(q, dev, n, dtype), _heads(gate, dev, n, dtype), half,
+               _ints(seq_len, dev, (n,)), groups, _ints(group_off, dev, (groups + 1,)), _ints(shared_len, dev, (groups,)),
+               max_shared, max_own, _table(chunk_ptrs, dev), table[1], k_off, v_off, 1 if kv_q8 else 0, window, sink,
+               out_ptr, _p(_dev(ws)), ws.numel())
     return out

@@ -740,3 +740,32 @@ def test_wrappers_refuse_tensors_of_another_kind():
             ops.gqa_prefill(*good[:at], bad, *good[at + 1:])
     with pytest.raises(ValueError):
         ops.gqa_prefill(*good[:2], ints(0, 2, 4), ints(40, 40), *good[4:])
+
+
+def test_wrappers_refuse_host_tensors():
+    from qwowl35_b200 import ops
+    t, i = torch.zeros(1, 10240), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(TypeError, match="device tensor"):
+        ops.attn_append(t, t, t, t, i, (32,), i, i, i, 0, 0)
+    with pytest.raises(TypeError, match="device tensor"):
+        ops.gqa_prefill(t, None, i, i, 1, 1, i, 0, 0)
+    with pytest.raises(TypeError, match="device tensor"):
+        ops.gqa_decode_shared(t, None, i, i, i, 1, 1, i, 0, 0)
+
+
+@pytest.mark.gpu
+def test_tensors_on_another_device_than_the_current_one():
+    """The calls run on their tensors' device and leave the current one as it was."""
+    from qwowl35_b200 import ops
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    cache = Cache([700], False, 2).fill([700], 3)
+    q, gt = some(5, 1, torch.float16), some(5, 2, torch.float16)
+    want = ops.gqa_prefill(q, gt, ints(0, 5), ints(700), 5, 700, cache.ptrs(), cache.k_off, cache.v_off)
+    raw = cache.raw.to("cuda:1")
+    table = torch.where(cache.ids >= 0, raw.data_ptr() + cache.ids * 4 * cache.plane, 0).to("cuda:1")
+    got = ops.gqa_prefill(q.to("cuda:1"), gt.to("cuda:1"), ints(0, 5).to("cuda:1"), ints(700).to("cuda:1"), 5, 700, table, cache.k_off,
+                          cache.v_off)
+    assert torch.cuda.current_device() == 0 and torch.equal(got.cpu(), want.cpu())
+    with pytest.raises(TypeError):
+        ops.gqa_prefill(q, gt.to("cuda:1"), ints(0, 5), ints(700), 5, 700, cache.ptrs(), cache.k_off, cache.v_off)
