@@ -36,6 +36,7 @@
 //
 // Work is split along the positions where there are few row tiles; the parts'
 // (m, l, O) go through the workspace and attn_join_kernel merges them.
+#include <algorithm>
 #include <cstdlib>
 #include <type_traits>
 
@@ -1056,14 +1057,23 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // The same plan for the workspace query and the launch.
 TilePlan plan_for(int n_row, int n_run, int max_run, int max_len, int max_own, bool shared) {
     TilePlan pl{};
-    pl.pair = !shared && max_run > TM_TOK;
-    const int toks = TM_TOK * (pl.pair ? 2 : 1), sms = kPlanSMs / (pl.pair ? 2 : 1);
+    // the most row tiles of `toks` tokens that the rows, divided into so many runs, can make
     const int runs = n_run < n_row ? n_run : n_row;
-    pl.tiles = (n_row - runs) / toks + runs;  // the most that rows divided into so many runs can make
+    auto row_tiles = [&](int toks) {
+        const long long most = shared ? n_row : (long long)n_run * ceil_div(max_run, toks);
+        return (int)std::min<long long>((n_row - runs) / toks + runs, most);
+    };
+    pl.tiles = row_tiles(TM_TOK);
     if (!shared) {
-        const long long most = (long long)n_run * ceil_div(max_run, toks);
-        if (most < pl.tiles) pl.tiles = (int)most;
-        const int units = pl.tiles * AKV, kv = ceil_div(max_len, kPlanTile);
+        // Pairs read and multiply with fewer pauses but take longer to set up: they pay from about two row tiles x
+        // 128 positions an SM on.  f16, pairs against single CTAs: 4 runs of 64 tokens 13.8 against 11.4 us, 64
+        // tokens at 4096 24.7 against 24.3, at 8128 28.1 against 31.2, at 32704 53.4 against 70.9, a prompt of 1024
+        // 24.7 against 28.2, of 8192 441 against 601; f32 alike (64 tokens at 32704 62.7 against 74.8).
+        const int kv = ceil_div(max_len, kPlanTile);
+        pl.pair = max_run > TM_TOK && (long long)pl.tiles * AKV * kv > 2 * kPlanSMs;
+        const int sms = kPlanSMs / (pl.pair ? 2 : 1);
+        if (pl.pair) pl.tiles = row_tiles(2 * TM_TOK);
+        const int units = pl.tiles * AKV;
         pl.ns = units >= sms ? 1 : sms / units;
         if (pl.ns > kv) pl.ns = kv;
         pl.each = ceil_div(kv, pl.ns);
