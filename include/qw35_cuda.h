@@ -185,8 +185,9 @@ int qw35_cuda_attn_append(uint32_t n_tok, const float *qkv, uint32_t qkv_stride,
 // seq_len[i]; the run's row t attends positions [0, seq_len[i] - run length + t],
 // cut by window and sink as in qw35_cuda_gqa_decode.  n_row is the number of rows
 // of q; rows outside every run are left as they were.  max_run and max_len are
-// upper bounds of a run's rows and of seq_len.  The cache rows of [0, seq_len[i])
-// have to be finite, masked or not; what lies behind them is not looked at.
+// upper bounds of a run's rows and of seq_len.  What a row does not attend does
+// not reach it, infinities and NaNs included; what lies behind seq_len[i] is not
+// looked at.
 uint64_t qw35_cuda_gqa_prefill_workspace_bytes(uint32_t n_row, uint32_t n_run, uint32_t max_run, uint32_t max_len);
 int qw35_cuda_gqa_prefill(uint32_t n_row, const void *q, const void *gate, uint32_t dtype, uint32_t n_run,
                           const int32_t *run_off, const int32_t *seq_len, uint32_t max_run, uint32_t max_len,
@@ -200,8 +201,7 @@ int qw35_cuda_gqa_prefill(uint32_t n_row, const void *q, const void *gate, uint3
 // [0, shared_len[g]) (read through the group's first table row); the rest of
 // their seq_len[i] positions are their own.  A sequence may end inside the
 // prefix.  Sequences of no group are left as they were.  max_shared and max_own
-// are upper bounds of shared_len and of seq_len[i] - shared_len[g].  The cache
-// rows in reach have to be finite, as above.
+// are upper bounds of shared_len and of seq_len[i] - shared_len[g].
 uint64_t qw35_cuda_gqa_decode_shared_workspace_bytes(uint32_t n_seq, uint32_t n_group, uint32_t max_shared,
                                                      uint32_t max_own);
 int qw35_cuda_gqa_decode_shared(uint32_t n_seq, const void *q, const void *gate, uint32_t dtype,

@@ -97,11 +97,13 @@ constexpr uint32_t kQlo = 384;  // TMEM columns of the lo half of Q
 constexpr int kMaxStages = 5;
 struct __align__(16) TileShared {
     uint64_t full[kMaxStages], ready[kMaxStages], empty[kMaxStages];
-    uint64_t s_full[2], p_full[2], pv_done, q_full, q_moved, o_full;
+    uint64_t s_full[2], p_full[2], pv_done, q_full, q_moved, o_full, looked;
     uint32_t tmem;
     int abort;
     int row0, nrow, kvh, table, part;  // this CTA's rows, kv head, chunk-table row, part number
     int lo, hi_max, hi_min, rs_max;    // positions [lo, hi) of the rows
+    int hi_all, rs_all;                // of a pair: hi_min and rs_max over both CTAs
+    int bad;                           // a V value that some row must not see is not finite
     int a0, n1, t2, begin, end;        // tile list: a0 .. a0+n1-1, then t2 ..; this CTA's share of it
     int hi[TM_TOK], sk[TM_TOK], rs[TM_TOK];
     float ex[2][2][TM_ROWS];           // row maxima (then sums) exchanged between the two column halves
@@ -123,21 +125,23 @@ __device__ __forceinline__ uint32_t cta_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// arrive on the leader's (rank 0's) copy of a barrier; MEM: this thread's (and its warp's) writes to memory go before it,
-// else only what a tcgen05 fence orders
+// arrive on a CTA's copy of a barrier; MEM: this thread's (and its warp's) writes to memory go before it, else only
+// what a tcgen05 fence orders
 template <bool MEM>
-__device__ __forceinline__ void arrive_leader(uint64_t *bar) {
+__device__ __forceinline__ void arrive_at(uint64_t *bar, int rank) {
     if constexpr (MEM)
         asm volatile(
-            "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
-            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+            "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\t"
+            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)), "r"(rank)
             : "memory");
     else
         asm volatile(
-            "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
-            "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+            "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\t"
+            "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)), "r"(rank)
             : "memory");
 }
+template <bool MEM>
+__device__ __forceinline__ void arrive_leader(uint64_t *bar) { arrive_at<MEM>(bar, 0); }
 template <bool PAIR>
 __device__ __forceinline__ void commit(uint64_t *bar) {  // to both CTAs' copies
     if constexpr (PAIR)
@@ -341,7 +345,7 @@ __device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan 
     const int row0 = w.row0;
     if (w.begin < 0 || row0 < 0 || row0 + nrow > p.n_row) nrow = 0;  // (offsets that make no sense)
     // lane = token of the CTA's tile; a pair walks the positions that either of its tiles needs
-    int lo = 0, hi_max = 0, rs_min = 0x7fffffff, sk_max = 0;
+    int lo = 0, hi_max = 0, rs_min = 0x7fffffff, sk_max = 0, hi_all = 0x7fffffff, rs_all = 0;
     for (int e = 0; e < CTAS; ++e) {
         const int tok = e * TM_TOK + lane;
         const bool real = tok < nrow;
@@ -362,11 +366,13 @@ __device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan 
         hi_max = max(hi_max, warp_max_i(hi));
         rs_min = min(rs_min, warp_min_i(real && hi > 0 ? rs : 0x7fffffff));
         sk_max = max(sk_max, warp_max_i(sk));
+        const int hi_min = warp_min_i(real ? hi : 0x7fffffff), rs_max = warp_max_i(rs);
+        hi_all = min(hi_all, hi_min);
+        rs_all = max(rs_all, rs_max);
         if (e == rank) {
             s.hi[lane] = hi;
             s.sk[lane] = sk;
             s.rs[lane] = rs;
-            const int hi_min = warp_min_i(real ? hi : 0x7fffffff), rs_max = warp_max_i(rs);
             if (lane == 0) {
                 s.hi_min = hi_min;
                 s.rs_max = rs_max;
@@ -389,7 +395,7 @@ __device__ __forceinline__ bool find_work(const AttnTileArgs &p, const TilePlan 
         s.kvh = kvh;
         s.table = p.shared_len ? (tail ? row0 : w.begin) : max(w.run, 0);
         s.part = tail ? pl.ns + split : split;
-        s.lo = lo; s.hi_max = hi_max;
+        s.lo = lo; s.hi_max = hi_max; s.hi_all = hi_all; s.rs_all = rs_all; s.bad = 0;
         s.a0 = a0; s.n1 = n1; s.t2 = t2;
         const int each = pl.each * (kPlanTile / TK);
         s.begin = min(total, split * each);
@@ -461,7 +467,7 @@ struct Loader {
     const AttnTileArgs &p;
     TileShared &s;
     uint32_t ring;
-    int tid, rank, lo, hi, n, slot = 0;
+    int tid, rank, lo, hi, n, rs_all, hi_all, slot = 0;
     uint32_t phase = 1;  // parity that the slot's last release has; the first round waits for none
 
     __device__ __forceinline__ TileRef ref(int i) const {  // 0: K(0); 2 j + 1: K(j + 1); 2 j + 2: V(j); the last: V(n - 1)
@@ -474,6 +480,55 @@ struct Loader {
         h.pos0 = t * G::TK + (h.v ? 0 : rank * G::KR);
         h.row0 = s.kvh * ACHUNK + h.pos0 % ACHUNK;
         return h;
+    }
+    // A probability of 0 does not keep an infinity or NaN out of a product, so V tiles that some row does not see all
+    // of are looked through; what is found sends the unit to attend_exactly().
+    __device__ __forceinline__ bool some_masked(int pos0) const { return pos0 < rs_all || min(pos0 + G::TK, hi) > hi_all; }
+    static __device__ __forceinline__ bool not_finite(const uint4 &v) {  // of 8 halves: an exponent of all ones
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) any |= (w[i] & 0x7c007c00u) + 0x04000400u;
+        return (any & 0x80008000u) != 0;
+    }
+    __device__ __forceinline__ void report() {  // in both CTAs: each one's dims reach the other's rows
+        *(volatile int *)&s.bad = 1;
+        if constexpr (PAIR)
+            asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tst.shared::cluster.u32 [a], %2;\n\t}" ::"r"(
+                             smem_u32(&s.bad)),
+                         "r"(rank ^ 1), "r"(1)
+                         : "memory");
+    }
+    // Once all loads are under way, from the cache again (looking tile by tile on the way cost a prompt 5%)
+    __device__ __forceinline__ void look(int t) {
+        const uint64_t base = p.chunk_ptrs[(size_t)s.table * p.max_chunks + t / (ACHUNK / G::TK)];
+        if (base == 0) return;
+        if constexpr (Q8) {
+            for (int i = tid; i < G::TK * 8; i += G::LOADERS * 32) {  // the d of block i % 8 of a position
+                const int pos = t * G::TK + i / 8;
+                if (pos < lo || pos >= hi) continue;
+                const uint8_t *row = reinterpret_cast<const uint8_t *>(base + p.v_off) + (size_t)(s.kvh * ACHUNK + pos % ACHUNK) * kKvQ8Row;
+                const uint32_t d = *reinterpret_cast<const unsigned short *>(row + 34 * (i % 8)) & 0x7fffu;
+                if (d >= 0x6000u) report();  // from 512 on, 127 d leaves the f16 range
+            }
+            return;
+        }
+        constexpr int RP = G::LOADERS * 32 / G::VP, N = G::TK / RP;
+        const int r0 = tid / G::VP, pos0 = t * G::TK;
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(base + p.v_off) +
+                             (size_t)(s.kvh * ACHUNK + pos0 % ACHUNK + r0) * (AHD * 2) + (rank * G::VP + tid % G::VP) * 16;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int pos = pos0 + r0 + i * RP;
+            if (pos >= lo && pos < hi) bad |= not_finite(*reinterpret_cast<const uint4 *>(src + (size_t)i * RP * AHD * 2));
+        }
+        if (bad) report();
+    }
+    __device__ __forceinline__ void look_through() {  // (tiles ascend: what is masked lies at the ends of the list)
+        int j = 0;
+        for (; j < n && tile_at(s, s.begin + j) * G::TK < rs_all; ++j) look(tile_at(s, s.begin + j));
+        for (int e = n - 1; e >= j && some_masked(tile_at(s, s.begin + e) * G::TK); --e) look(tile_at(s, s.begin + e));
     }
     // next free stage
     __device__ __forceinline__ int acquire(int stage) {
@@ -569,7 +624,13 @@ struct Loader {
                 else copy<false>(h, i);
                 h = next;
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+        look_through();
+        if constexpr (!Q8) asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        if ((tid & 31) == 0) {
+            mbar_arrive(&s.looked);
+            if constexpr (PAIR) arrive_at<true>(&s.looked, rank ^ 1);
         }
     }
 };
@@ -681,6 +742,51 @@ __device__ __forceinline__ void relay(TileShared &s, int rank) {
     }
 }
 
+// Row r of this CTA on the CUDA cores, from the cache itself and over the attended positions alone: the unit's values
+// hold infinities or NaNs that the row may have to be kept from.  8 dims a lane; o unscaled, m in log2 units.
+template <typename T, bool Q8>
+__device__ __forceinline__ void attend_exactly(const AttnTileArgs &p, const TileShared &s, int r, int tk, float *o, float &m, float &l) {
+    const int lane = threadIdx.x & 31, tok = r / AGRP;
+    const int hi = s.hi[tok], sk = s.sk[tok], rs = s.rs[tok];
+    const float c = p.scale * kLog2e;
+    float q[8], k[8], v[8];
+    get8(static_cast<const T *>(p.q) + ((size_t)(s.row0 + tok) * AH + s.kvh * AGRP + r % AGRP) * AHD + lane * 8, q);
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = 0.0f;
+    for (int j = s.begin; j < s.end; ++j) {
+        const int t = tile_at(s, j);
+        const uint64_t base = p.chunk_ptrs[(size_t)s.table * p.max_chunks + t * tk / ACHUNK];
+        for (int pos = t * tk; pos < (t + 1) * tk && base; ++pos) {
+            if (pos < s.lo || pos >= hi || (pos >= sk && pos < rs)) continue;
+            const size_t row = (size_t)s.kvh * ACHUNK + pos % ACHUNK;
+            auto values = [&](uint64_t plane, float *x) {
+                if constexpr (Q8) {
+                    const uint8_t *blk = reinterpret_cast<const uint8_t *>(plane) + row * kKvQ8Row + 34 * (lane >> 2);
+                    const float d = __half2float(*reinterpret_cast<const __half *>(blk));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = d * (float)(int8_t)blk[2 + 8 * (lane & 3) + i];
+                } else {
+                    get8(reinterpret_cast<const __half *>(plane) + row * AHD + lane * 8, x);
+                }
+            };
+            values(base + p.k_off, k);
+            values(base + p.v_off, v);
+            float x = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x = fmaf(q[i], k[i], x);
+            x = warp_sum(x) * c;
+            const float nm = fmaxf(m, x);
+            const float a = m == -INFINITY ? 0.0f : ex2(m - nm), e = x == -INFINITY ? 0.0f : ex2(x - nm);
+            l = l * a + e;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = (m == -INFINITY ? 0.0f : o[i] * a) + (e == 0.0f ? 0.0f : e * v[i]);
+            m = nm;
+        }
+    }
+}
+
 // ---- the kernel ---------------------------------------------------------------------
 template <bool HL, bool Q8, bool PAIR>
 __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_kernel(AttnTileArgs p, TilePlan pl) {
@@ -712,6 +818,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
         mbar_init(&s.q_full, SOFT_WARPS * G::CTAS);
         mbar_init(&s.q_moved, SOFT_WARPS);
         mbar_init(&s.o_full, 1);
+        mbar_init(&s.looked, G::LOADERS * G::CTAS);
         s.abort = 0;
         fence_barrier_init();
     }
@@ -733,7 +840,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
 
     if (warp >= SOFT_WARPS && warp < MMA_WARP) {
         set_regs<G::SPLIT, G::LOAD_REGS, false>();
-        Loader<HL, Q8, PAIR> ld{p, s, sbase + G::QB, tid - SOFT_WARPS * 32, rank, s.lo, s.hi_max, s.end - s.begin};
+        Loader<HL, Q8, PAIR> ld{p, s, sbase + G::QB, tid - SOFT_WARPS * 32, rank, s.lo, s.hi_max, s.end - s.begin, s.rs_all, s.hi_all};
         ld.run();
     } else if (warp >= MMA_WARP) {
         set_regs<G::SPLIT, G::REST_REGS, false>();
@@ -928,6 +1035,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
         fetch_gates(warp);
         if (n > 0) {
             tw(&s.o_full, 0, s, 128u);
+            tw(&s.looked, 0, s, 128u);
             tc_fence_after();
         }
         float *buf = reinterpret_cast<float *>(smem);
@@ -936,6 +1044,18 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
             s.ex[n & 1][grp][row] = l;
             named_sync(1 + quarter, 64);
             l += s.ex[n & 1][grp ^ 1][row];
+        }
+        if (n > 0 && *(volatile int *)&s.bad) {
+            for (int r = warp; r < rows; r += SOFT_WARPS) {
+                float o[8], rm, rl;
+                attend_exactly<T, Q8>(p, s, r, G::TK, o, rm, rl);
+                const float inv = join ? 1.0f : (rl == 0.0f ? 0.0f : 1.0f / rl);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = inv == 0.0f ? 0.0f : o[i] * inv;
+                put8(buf + r * BROW + lane * 8, o);
+                if (join && lane == 0) static_cast<float2 *>(p.ws)[head_row(r) * parts + s.part] = make_float2(rm, rl);
+            }
+        } else if (busy) {
             const float inv = join ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
             if (n > 0) {
 #pragma unroll

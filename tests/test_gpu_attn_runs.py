@@ -379,6 +379,78 @@ def test_prefill_flat_and_peaked_scores(half, scale):
     check_rows(out, [(r, *attend(q[r], gt[r], k, v, 831 + r), 831 + r) for r in range(0, 70, 7)], half, False)
 
 
+def poison(cache, i, positions, value, planes=(0, 1)):
+    """Writes `value` into a few dims of K and V (q8_0: as a block's d) at positions of sequence i."""
+    rows = cache.rows()
+    for n, pos in enumerate(positions):
+        part = rows[int(cache.ids[i, pos // CH])]
+        for plane in planes:
+            for head in range(KV):
+                if cache.q8:
+                    part[plane, head, pos % CH, (3 * n + head) % 8, :2] = torch.tensor([value], dtype=torch.float16).view(torch.uint8).cuda()
+                else:
+                    part[plane, head, pos % CH, (37 * n + 5 * head) % D] = value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("inf"), float("nan"), -float("inf")])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q8", [False, True])
+def test_prefill_keeps_what_a_row_does_not_attend_from_it(value, half, q8):
+    """Infinities and NaNs at later tokens of the run and outside the window reach only the rows that attend them."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    for ctx, rows, at, window, sink in ((300, 40, (320, 339), 0, 0), (0, 300, (150, 151, 290), 0, 0), (900, 200, (1, 40, 500, 1050), 120, 3),
+                                          (900, 200, (40, 500, 1050), 120, 3)):
+        n = ctx + rows
+        cache = Cache([n], q8, 5).fill([n], 6)
+        poison(cache, 0, at, value)
+        q, gt = some(rows, 1, kind), some(rows, 2, kind, 1.0)
+        for r0 in (0, rows - 3):  # as one run, and its last rows alone (split along the positions)
+            out = ops.gqa_prefill(q[r0:], gt[r0:], ints(0, rows - r0), ints(n), rows - r0, n, cache.ptrs(), cache.k_off, cache.v_off,
+                                  window=window, sink=sink, kv_q8=q8)
+            k, v = cache.sequence(0, n)
+            clean, hit = [], []
+            for r in sorted({r0, r0 + 1, r0 + 2, *range(r0, rows, 7), *(p - ctx + d for p in at for d in (-1, 0, 1) if r0 <= p - ctx + d < rows)}):
+                length = ctx + r + 1
+                few = min(sink, length)
+                seen = [p for p in at if p < length and (window <= 0 or few + window >= length or p < few or p >= length - window)]
+                (hit if seen else clean).append(r)
+                if not seen:
+                    o, a, s = attend(q[r], gt[r], k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0), length, window, sink)
+                    check_rows(out, [(r - r0, o, a, s, length)], half, q8)
+            assert clean or r0 or 1 in at  # (position 1 is a sink: every row attends it)
+            for r in hit:
+                assert not torch.isfinite(out[r - r0]).all()
+    assert _lib.lib().qw35_cuda_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8", [(False, False), (True, False), (False, True)])
+def test_shared_keeps_what_a_sequence_does_not_attend_from_it(half, q8):
+    """A sequence that ends inside the prefix, and windows that leave some of it out, beside others that see it all."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    lens, shared = [700, 130, 900, 333], 640
+    for at, window in (((400, 639), 0), ((10, 200), 300)):
+        cache = Cache([900] * 4, q8, 5).fill([900] * 4, 6)
+        poison(cache, 0, at, float("nan"))
+        cache.ids[1:, :shared // CH] = cache.ids[0, :shared // CH]
+        rows = cache.rows()
+        for j in range(1, 4):
+            rows[int(cache.ids[j, 2])][:, :, :128] = rows[int(cache.ids[0, 2])][:, :, :128]
+        q, gt = some(4, 1, kind), some(4, 2, kind, 1.0)
+        out = ops.gqa_decode_shared(q, gt, ints(*lens), ints(0, 4), ints(shared), shared, 260, cache.ptrs(), cache.k_off, cache.v_off,
+                                    window=window, kv_q8=q8)
+        for i, length in enumerate(lens):
+            seen = [p for p in at if p < length and (window <= 0 or p >= length - window)]
+            if seen:
+                assert not torch.isfinite(out[i]).all()
+            else:
+                k, v = cache.sequence(i, length)
+                check_rows(out, [(i, *attend(q[i], gt[i], k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0), length, window), length)], half, q8)
+
+
 # ---- shared prefixes -----------------------------------------------------------------------
 
 def shared_case(groups, half, q8, window=0, sink=0, gate=True, seed=0, max_own=None):
