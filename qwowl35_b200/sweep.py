@@ -201,10 +201,51 @@ def attn_pre_b32(device) -> None:
         ops.attn_preprocess(qkv, qn, kn, freq, pos, table, 0, plane * 2)
 
 
+def _cache(device, seqs: int, chunks: int, shared: int = 0):
+    """f16 chunks of one layer and the chunk table [seqs, chunks]; the first `shared` chunks are everybody's."""
+    plane = 4 * 256 * 256
+    pool = torch.randn(shared + seqs * (chunks - shared), 2 * plane, device=device, dtype=torch.float16)
+    own = torch.arange(seqs * (chunks - shared)).view(seqs, -1) + shared
+    table = torch.cat([torch.arange(shared).expand(seqs, -1), own], 1) * (4 * plane) + pool.data_ptr()
+    return pool, table.contiguous().to(device), 2 * plane
+
+
+def append_4096(device) -> None:
+    """4,096 tokens of one sequence into the cache, rotary positions on three axes, f16 q and gate."""
+    n = 4096
+    pool, table, v_off = _cache(device, 1, n // 256)
+    qkv = torch.randn(n, 16 * 512 + 2048, device=device)
+    w, freq = torch.ones(256, device=device), torch.pow(1.0e7, -torch.arange(0, 64, 2, device=device, dtype=torch.float32) / 64.0)
+    pos = torch.arange(n, dtype=torch.int32, device=device)
+    for _ in range(3):
+        ops.attn_append(qkv, w, w, freq, pos.expand(3, -1).contiguous(), (11, 11, 10), torch.zeros_like(pos), pos, table, 0, v_off,
+                        dtype=torch.float16)
+
+
+def prefill_4096(device) -> None:
+    """Causal attention of a 4,096-token prompt, f16."""
+    n = 4096
+    pool, table, v_off = _cache(device, 1, n // 256)
+    q, gate = (torch.randn(n, 16, 256, device=device).half() for _ in range(2))
+    off, lens = (torch.tensor(v, dtype=torch.int32, device=device) for v in ([0, n], [n]))
+    for _ in range(3):
+        ops.gqa_prefill(q, gate, off, lens, n, n, table, 0, v_off)
+
+
+def shared_b32_ctx16384(device) -> None:
+    """A decode step of 32 sequences behind 16,384 shared positions with 256 of their own, f32."""
+    b, shared, own = 32, 16384, 256
+    pool, table, v_off = _cache(device, b, (shared + own) // 256, shared // 256)
+    q, gate = (torch.randn(b, 16, 256, device=device) for _ in range(2))
+    off, pre, lens = (torch.tensor(v, dtype=torch.int32, device=device) for v in ([0, b], [shared], [shared + own] * b))
+    for _ in range(3):
+        ops.gqa_decode_shared(q, gate, lens, off, pre, shared, own, table, 0, v_off)
+
+
 CASES = {"gateup_gf4_b32": gateup_gf4_b32, "matvec_q8_0_b1": matvec_q8_0_b1, "deltanet_b1": deltanet_b1,
          "deltanet_b32": deltanet_b32, "attn_pre_b32": attn_pre_b32, "gateup_gf4_b1": gateup_gf4_b1, "matvec_gf4_b1": matvec_gf4_b1,
-         "matvec_q8_0_b32": matvec_q8_0_b32, "gqa_b8_ctx4096": gqa_b8_ctx4096}
-
+         "matvec_q8_0_b32": matvec_q8_0_b32, "gqa_b8_ctx4096": gqa_b8_ctx4096, "append_4096": append_4096,
+         "prefill_4096": prefill_4096, "shared_b32_ctx16384": shared_b32_ctx16384}
 
 
 def main(argv: list[str]) -> int:
