@@ -372,13 +372,13 @@ static bool tile_args(qw35::AttnTileArgs &a, uint32_t n_row, const void *q, cons
     return true;
 }
 
-// Limits of the size queries too: rows and runs within a grid, lengths within the table's.
+// Limits of the size queries too: some work, rows and runs within a grid, lengths within the table's.
 static bool tile_sizes_ok(uint32_t n_row, uint32_t n_run, uint64_t len) {
-    return n_row <= (1u << 24) && n_run <= 65535 && len <= (1u << 29);
+    return n_row > 0 && n_row <= (1u << 24) && n_run > 0 && n_run <= 65535 && len <= (1u << 29);
 }
 
 uint64_t qw35_cuda_gqa_prefill_workspace_bytes(uint32_t n_row, uint32_t n_run, uint32_t max_run, uint32_t max_len) {
-    if (!tile_sizes_ok(n_row, n_run, max_len)) return 0;
+    if (max_run == 0 || max_run > n_row || max_len == 0 || !tile_sizes_ok(n_row, n_run, max_len)) return 0;
     return qw35::attn_tile_workspace_bytes((int)n_row, (int)n_run, (int)max_run, (int)max_len, 0);
 }
 
@@ -405,7 +405,9 @@ int qw35_cuda_gqa_prefill(uint32_t n_row, const void *q, const void *gate, uint3
 
 uint64_t qw35_cuda_gqa_decode_shared_workspace_bytes(uint32_t n_seq, uint32_t n_group, uint32_t max_shared,
                                                      uint32_t max_own) {
-    if (!tile_sizes_ok(n_seq, n_group, max_shared) || !tile_sizes_ok(n_seq, n_group, max_own)) return 0;
+    if ((max_shared == 0 && max_own == 0) || n_seq > 65535 || !tile_sizes_ok(n_seq, n_group, max_shared) ||
+        !tile_sizes_ok(n_seq, n_group, max_own))
+        return 0;
     return qw35::attn_tile_workspace_bytes((int)n_seq, (int)n_group, 0, (int)max_shared, (int)max_own);
 }
 

@@ -753,6 +753,34 @@ def test_calls_without_rows_do_nothing():
     _lib.call("qw35_cuda_gqa_decode_shared", *_shared_args(n=0))
 
 
+@pytest.mark.parametrize("sizes", [(0, 0, 0, 0), (0, 1, 1, 1), (4, 0, 1, 5), (4, 1, 0, 5), (4, 1, 1, 0), (4, 1, 5, 5),
+                                   (4, 1, 2 ** 32 - 1, 5), (4, 1, 2 ** 31, 5)])
+def test_prefill_sizes_without_work_need_no_workspace(sizes):
+    assert _lib.lib().qw35_cuda_gqa_prefill_workspace_bytes(*sizes) == 0
+
+
+@pytest.mark.parametrize("sizes", [(0, 0, 0, 0), (0, 1, 1, 1), (4, 0, 1, 5), (4, 1, 0, 0), (65536, 1, 1, 5)])
+def test_shared_sizes_without_work_need_no_workspace(sizes):
+    assert _lib.lib().qw35_cuda_gqa_decode_shared_workspace_bytes(*sizes) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+def test_wrappers_take_batches_without_rows(half):
+    from qwowl35_b200 import ops
+    cache = Cache([40], False, 5).fill([40], 6)
+    kind = torch.float16 if half else torch.float32
+    q, one = some(0, 1, kind), some(1, 1, kind)
+    at = (cache.ptrs(), cache.k_off, cache.v_off)
+    assert ops.gqa_prefill(q, q, ints(0, 0), ints(40), 0, 40, *at).shape == (0, H * D)
+    assert ops.gqa_prefill(q, None, ints(0), ints(), 0, 0, *at).shape == (0, H * D)
+    assert ops.gqa_decode_shared(q, q, ints(), ints(0, 0), ints(8), 8, 32, *at).shape == (0, H * D)
+    out = torch.full((1, H * D), 5.0, dtype=kind, device="cuda")  # a row of no group
+    ops.gqa_decode_shared(one, one, ints(40), ints(0), ints(), 0, 0, *at, out=out)
+    ops.gqa_prefill(one, one, ints(0), ints(), 0, 0, *at, out=out)
+    assert bool((out == 5).all()) and _lib.lib().qw35_cuda_device_error() == 0
+
+
 def _prefill_args(**over):
     a = dict(n=4, q=16, gate=None, dtype=0, runs=1, off=16, len=16, max_run=4, max_len=100, table=16, chunks=1, k=0, v=1 << 19, kv=0,
              window=0, sink=0, out=16, ws=16, bytes=1 << 40)
