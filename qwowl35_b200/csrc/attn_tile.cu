@@ -1137,7 +1137,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_join_kernel(AttnTileArgs
             w[k] = 0.0f;
             if (i < parts) {
                 const float2 t = ml[i];
-                if (t.x != -INFINITY) {  // (an empty part has no values)
+                if (t.x != -INFINITY || t.y != 0.0f) {  // (an empty part has no values; one of NaN scores has a NaN sum)
                     w[k] = ex2(t.x - mx);
                     l = fmaf(w[k], t.y, l);
                     get8(acc + (size_t)i * AHD, v[k]);
@@ -1163,7 +1163,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_join_kernel(AttnTileArgs
         for (int e = 0; e < 8; ++e) o[e] += t[e];
         l += part_l[w];
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         o[e] *= inv;

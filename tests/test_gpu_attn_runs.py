@@ -451,6 +451,46 @@ def test_shared_keeps_what_a_sequence_does_not_attend_from_it(half, q8):
                 check_rows(out, [(i, *attend(q[i], gt[i], k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0), length, window), length)], half, q8)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("ctx,rows", [(4000, 5), (300, 200), (9000, 70)])
+def test_prefill_nan_queries_and_keys_come_out(half, q8, ctx, rows):
+    """A NaN in a head's q makes that head's row NaN and no other; keys that are NaN over whole parts make every row NaN."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    n = ctx + rows
+    cache = Cache([n], q8, 5).fill([n], 6)
+    q, gt = some(rows, 1, kind), some(rows, 2, kind, 1.0)
+    r, h = rows // 2, 5
+    args = (gt, ints(0, rows), ints(n), rows, n, cache.ptrs(), cache.k_off, cache.v_off)
+    q[r, h, 77] = float("nan")
+    out = ops.gqa_prefill(q, *args, kv_q8=q8).view(rows, H, D)
+    bad = out.isnan()
+    assert bool(bad[r, h].all()) and int(bad.sum()) == D
+    q[r, h, 77] = 0.5
+    part = cache.rows()[int(cache.ids[0, 0]), 0]
+    if q8:
+        part[..., :2] = torch.tensor([0, 0x7e], dtype=torch.uint8, device="cuda")
+    else:
+        part.fill_(float("nan"))
+    assert bool(ops.gqa_prefill(q, *args, kv_q8=q8).isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8", [(False, False), (True, False), (False, True)])
+def test_shared_nan_queries_come_out(half, q8):
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    cache = Cache([900] * 4, q8, 5).fill([900] * 4, 6)
+    cache.ids[1:, :2] = cache.ids[0, :2]
+    q, gt = some(4, 1, kind), some(4, 2, kind, 1.0)
+    q[2, 9, 0] = float("nan")
+    out = ops.gqa_decode_shared(q, gt, ints(900, 600, 700, 513), ints(0, 4), ints(512), 512, 388, cache.ptrs(), cache.k_off, cache.v_off,
+                                kv_q8=q8).view(4, H, D)
+    assert bool(out[2, 9].isnan().all()) and int(out.isnan().sum()) == D
+
+
 # ---- shared prefixes -----------------------------------------------------------------------
 
 def shared_case(groups, half, q8, window=0, sink=0, gate=True, seed=0, max_own=None):
