@@ -181,6 +181,13 @@ def _heads(t, dev, n, dtype):
     return t.data_ptr()
 
 
+def _workspace(t, dev):
+    """A workspace: bytes on the tensors' device."""
+    if t.dtype is not torch.uint8 or t.get_device() != dev or not t.is_contiguous():
+        raise TypeError(f"contiguous uint8 workspace on cuda:{dev} expected, got {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
 def _head_dtype(dtype):
     if dtype is torch.float32:
         return 0
@@ -227,8 +234,8 @@ def attn_append(qkv, q_norm_w, k_norm_w, rope_freq, rope_pos, sections, tok_seq,
     """
     dev = _device_of(qkv)
     shape = qkv.shape
-    if qkv.dtype is not torch.float32 or len(shape) != 2 or shape[1] < 10240 or qkv.stride(1) != 1:
-        raise TypeError("qkv must be a float32 device tensor [n, >= 10240] with contiguous rows")
+    if qkv.dtype is not torch.float32 or len(shape) != 2 or shape[1] < 10240 or qkv.stride(1) != 1 or qkv.stride(0) >= 1 << 32:
+        raise TypeError("qkv must be a float32 device tensor [n, >= 10240] with contiguous rows less than 2^32 values apart")
     n, axes, half = shape[0], len(sections), _head_dtype(dtype)
     if q is None:
         q = qkv.new_empty((n, 16, 256), dtype=dtype)
@@ -275,7 +282,7 @@ def gqa_prefill(q, gate, run_off, seq_len, max_run, max_len, chunk_ptrs, k_off, 
         ws = q.new_empty(L.qw35_cuda_gqa_prefill_workspace_bytes(n, runs, max_run, max_len), dtype=torch.uint8)
     _on_device(dev, L.qw35_cuda_gqa_prefill, n, _heads(q, dev, n, dtype), _heads(gate, dev, n, dtype), half, runs,
                _ints(run_off, dev, (runs + 1,)), _ints(seq_len, dev, (runs,)), max_run, max_len, _table(chunk_ptrs, dev),
-               table[1], k_off, v_off, 1 if kv_q8 else 0, window, sink, out_ptr, _p(_dev(ws)), ws.numel())
+               table[1], k_off, v_off, 1 if kv_q8 else 0, window, sink, out_ptr, _workspace(ws, dev), ws.numel())
     return out
 
 
@@ -306,5 +313,5 @@ def gqa_decode_shared(q, gate, seq_len, group_off, shared_len, max_shared, max_o
     _on_device(dev, L.qw35_cuda_gqa_decode_shared, n, _heads(q, dev, n, dtype), _heads(gate, dev, n, dtype), half,
                _ints(seq_len, dev, (n,)), groups, _ints(group_off, dev, (groups + 1,)), _ints(shared_len, dev, (groups,)),
                max_shared, max_own, _table(chunk_ptrs, dev), table[1], k_off, v_off, 1 if kv_q8 else 0, window, sink,
-               out_ptr, _p(_dev(ws)), ws.numel())
+               out_ptr, _workspace(ws, dev), ws.numel())
     return out

@@ -882,6 +882,35 @@ def test_wrappers_refuse_tensors_of_another_kind():
         ops.gqa_prefill(*good[:2], ints(0, 2, 4), ints(40, 40), *good[4:])
 
 
+@pytest.mark.gpu
+def test_wrappers_refuse_workspaces_elsewhere():
+    from qwowl35_b200 import ops
+    cache = Cache([40], False, 5).fill([40], 6)
+    q = some(4, 1, torch.float32)
+    at = (cache.ptrs(), cache.k_off, cache.v_off)
+    n = max(ops.gqa_prefill_workspace(4, 1, 4, 40).numel(), ops.gqa_decode_shared_workspace(1, 1, 8, 32).numel())
+    bad = [torch.empty(n, dtype=torch.uint8), torch.empty(n, dtype=torch.float32, device="cuda"),
+           torch.empty(2 * n, dtype=torch.uint8, device="cuda")[::2]]
+    if torch.cuda.device_count() > 1:
+        bad.append(torch.empty(n, dtype=torch.uint8, device="cuda:1"))
+    for ws in bad:
+        with pytest.raises(TypeError, match="workspace"):
+            ops.gqa_prefill(q, q, ints(0, 4), ints(40), 4, 40, *at, ws=ws)
+        with pytest.raises(TypeError, match="workspace"):
+            ops.gqa_decode_shared(q[:1], q[:1], ints(40), ints(0, 1), ints(8), 8, 32, *at, ws=ws)
+
+
+@pytest.mark.gpu
+def test_append_refuses_rows_too_far_apart():
+    """The C call takes the stride in 32 bits: 2^32 + 10240 must not become 10240."""
+    from qwowl35_b200 import ops
+    cache = Cache([40], False, 5)
+    qkv = torch.empty(2 ** 32 + 2 * 10240, device="cuda").as_strided((2, 10240), (2 ** 32 + 10240, 1))
+    w = torch.ones(256, device="cuda")
+    with pytest.raises(TypeError, match="apart"):
+        ops.attn_append(qkv, w, w, FREQ.cuda(), ints(0, 1)[None], (32,), ints(0, 0), ints(0, 1), cache.ptrs(), cache.k_off, cache.v_off)
+
+
 def test_wrappers_refuse_host_tensors():
     from qwowl35_b200 import ops
     t, i = torch.zeros(1, 10240), torch.zeros(2, dtype=torch.int32)
