@@ -245,8 +245,19 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo = pack2(a - f.x, b - f.y);
 }
 
-// 1 / (1 + e^-x), a few units of 2^-24 off (sigmoid_f's exact division and exponential cost an epilogue 4 us)
-__device__ __forceinline__ float sigmoid_fast(float x) { return __fdividef(1.0f, 1.0f + ex2(fmaxf(-x * kLog2e, -126.0f))); }
+// 1 / (1 + e^-x) to 2^-20 (ex2 and the quotient 2^-22 each; sigmoid_f's exact division and exponential cost an epilogue
+// 4 us); below the smallest normal number 0, and NaN for NaN.  t = -x log2 e is rounded, by up to 2^-18 for gates of
+// -80, so what it lost (r, with the rest of log2 e) enters as a factor 1 + r ln 2.  The ends, beyond which f32 has 0 or
+// 1, keep e within what __fdividef divides by (2^126) and infinities out of r.
+__device__ __forceinline__ float sigmoid_fast(float x) {
+    float z;
+    asm("{\n\t.reg .f32 a;\n\tmax.NaN.f32 a, %1, %2;\n\tmin.NaN.f32 %0, a, %3;\n\t}" : "=f"(z) : "f"(x), "f"(-87.33654f), "f"(88.0f));
+    const float t = -z * kLog2e;
+    const float r = fmaf(-z, 1.92596303e-8f, fmaf(-z, kLog2e, -t));
+    const float e = ex2(t);
+    const float y = __fdividef(1.0f, 1.0f + fmaf(e, r * 0.693147181f, e));
+    return x < -87.33654f ? 0.0f : y;
+}
 
 // 8 consecutive values of a row, 16-byte aligned
 __device__ __forceinline__ void get8(const float *p, float *v) {

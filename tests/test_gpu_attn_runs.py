@@ -938,3 +938,61 @@ def test_tensors_on_another_device_than_the_current_one():
     assert torch.cuda.current_device() == 0 and torch.equal(got.cpu(), want.cpu())
     with pytest.raises(TypeError):
         ops.gqa_prefill(q, gt.to("cuda:1"), ints(0, 5), ints(700), 5, 700, cache.ptrs(), cache.k_off, cache.v_off)
+
+
+# ---- gates, and values that are not finite --------------------------------------------------------------
+
+GATES = [float("nan"), float("inf"), float("-inf"), 0.0, -0.5, 3.0, -5.0, 12.0, -12.0, 20.0, -20.0, 60.0, -60.0, -80.0, -86.0, 86.0, -88.0,
+         88.0, -104.0, 104.0, -300.0, 300.0, -60000.0, 60000.0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("shared", [False, True])
+def test_gates_of_every_size(half, shared):
+    """One attended position: the output is its value times the gate's sigmoid, to 2^-20 (an exponential and a quotient of
+    2^-22 each, four roundings of 2^-24) and nothing below the smallest normal number; NaN gates come out as NaN."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    n = 40
+    cache = Cache([1] * n, False, 5).fill([1] * n, 6)
+    q = some(n, 1, kind)
+    g = torch.Generator("cuda").manual_seed(3)
+    gate = (torch.rand(n, H, D, device="cuda", generator=g) * 220 - 110).to(kind)
+    gate[::2] = torch.tensor(GATES, device="cuda").to(kind).repeat(H * D)[:H * D].view(H, D)
+    at = (cache.ptrs(), cache.k_off, cache.v_off)
+    if shared:  # (parts are joined)
+        out = ops.gqa_decode_shared(q, gate, ints(*[1] * n), ints(*range(n + 1)), ints(*[i % 2 for i in range(n)]), 1, 1, *at)
+    else:
+        out = ops.gqa_prefill(q, gate, ints(*range(n + 1)), ints(*[1] * n), 1, 1, *at)
+    v = torch.stack([cache.sequence(i, 1)[1][:, 0] for i in range(n)]).repeat_interleave(H // KV, 1)
+    want, got = v * torch.sigmoid(gate.double()), out.view(n, H, D).double()
+    nan = gate.isnan()
+    assert bool(got[nan].isnan().all()) and bool(torch.isfinite(got[~nan]).all())
+    tol = (2.0 ** -20 + (2.0 ** -11 if half else 0)) * want.abs() + 2.0 ** -126 * v.abs() + (2.0 ** -25 if half else 2.0 ** -149)
+    err = ((got - want).abs() / tol)[~nan]
+    assert float(err.max()) <= 1.0, float(err.max())
+    assert bool((got[gate == float("-inf")] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("ctx,rows", [(300, 20), (4000, 5), (9000, 70)])
+def test_prefill_nan_and_infinite_gates(half, q8, ctx, rows):
+    """In one piece, joined, and on CTA pairs: a gate's NaN stays at its own value."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    n = ctx + rows
+    cache = Cache([n], q8, 5).fill([n], 6)
+    q, gt = some(rows, 1, kind), some(rows, 2, kind, 1.0)
+    args = (ints(0, rows), ints(n), rows, n, cache.ptrs(), cache.k_off, cache.v_off)
+    want = ops.gqa_prefill(q, gt, *args, kv_q8=q8).view(rows, H, D)
+    bare = ops.gqa_prefill(q, None, *args, kv_q8=q8).view(rows, H, D)
+    gt[1::3, 3, 7::11] = float("nan")
+    gt[::2, 9, 5::13] = float("inf")
+    gt[::2, 15, 2::3] = -float("inf")
+    got = ops.gqa_prefill(q, gt, *args, kv_q8=q8).view(rows, H, D)
+    assert torch.equal(got.isnan(), gt.isnan())
+    assert torch.equal(got[gt == float("inf")], bare[gt == float("inf")]) and bool((got[gt == -float("inf")] == 0).all())
+    same = torch.isfinite(gt)
+    assert torch.equal(got[same], want[same])
