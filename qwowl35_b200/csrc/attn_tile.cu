@@ -56,6 +56,7 @@ constexpr int kPlanSMs = 148;
 constexpr int kPlanTile = 128;           // positions by which work is divided: a whole number of any variant's tiles
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kShift = 7.0f, kSlack = 8.0f;  // log2: offset of P, growth of the maximum before O is rescaled
+constexpr float kNoScore = -3.0e38f;  // the maximum that a part leaves which has values but no finite score (an empty one: -infinity)
 
 template <bool HL, bool Q8, bool PAIR>
 struct TileGeo {
@@ -789,10 +790,11 @@ __device__ __forceinline__ void attend_exactly(const AttnTileArgs &p, const Tile
             for (int i = 0; i < 8; ++i) x = fmaf(q[i], k[i], x);
             x = warp_sum(x) * c;
             const float nm = fmaxf(m, x);
-            const float a = m == -INFINITY ? 0.0f : ex2(m - nm), e = x == -INFINITY ? 0.0f : ex2(x - nm);
+            // (before the first finite score l and o are 0, or NaN and have to stay so; nor may a weight of 0 hide one)
+            const float a = m == -INFINITY ? 1.0f : ex2(m - nm), e = x == -INFINITY ? 0.0f : ex2(x - nm);
             l = l * a + e;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = (m == -INFINITY ? 0.0f : o[i] * a) + (e == 0.0f ? 0.0f : e * v[i]);
+            for (int i = 0; i < 8; ++i) o[i] = o[i] * a + e * v[i];
             m = nm;
         }
     }
@@ -1062,9 +1064,9 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 attend_exactly<T, Q8>(p, s, r, G::TK, o, rm, rl);
                 const float inv = join ? 1.0f : (rl == 0.0f ? 0.0f : 1.0f / rl);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = inv == 0.0f ? 0.0f : o[i] * inv;
+                for (int i = 0; i < 8; ++i) o[i] *= inv;
                 put8(buf + r * BROW + lane * 8, o);
-                if (join && lane == 0) static_cast<float2 *>(p.ws)[head_row(r) * parts + s.part] = make_float2(rm, rl);
+                if (join && lane == 0) static_cast<float2 *>(p.ws)[head_row(r) * parts + s.part] = make_float2(fmaxf(rm, kNoScore), rl);
             }
         } else if (busy) {
             const float inv = join ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
@@ -1082,7 +1084,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 }
             }
             if (join && real && grp == 0)
-                static_cast<float2 *>(p.ws)[head_row(row) * parts + s.part] = make_float2(m == -INFINITY ? m : fmaf(m, c, -kShift), l);
+                static_cast<float2 *>(p.ws)[head_row(row) * parts + s.part] = make_float2(m == -INFINITY ? kNoScore : fmaf(m, c, -kShift), l);
         }
         named_sync(9, SOFT_WARPS * 32);
         float *acc = reinterpret_cast<float *>(static_cast<float2 *>(p.ws) + (size_t)p.n_row * AH * parts);
@@ -1142,13 +1144,15 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_join_kernel(AttnTileArgs
     constexpr int B = 8;
     for (int i0 = warp; i0 < parts; i0 += JOIN_WARPS * B) {
         float w[B], v[B][8];
+        bool there[B];
 #pragma unroll
         for (int k = 0; k < B; ++k) {
             const int i = i0 + k * JOIN_WARPS;
-            w[k] = 0.0f;
+            there[k] = false;
             if (i < parts) {
                 const float2 t = ml[i];
-                if (t.x != -INFINITY || t.y != 0.0f) {  // (an empty part has no values; one of NaN scores has a NaN sum)
+                if (t.x != -INFINITY) {  // (an empty part has no values)
+                    there[k] = true;
                     w[k] = ex2(t.x - mx);
                     l = fmaf(w[k], t.y, l);
                     get8(acc + (size_t)i * AHD, v[k]);
@@ -1157,7 +1161,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_join_kernel(AttnTileArgs
         }
 #pragma unroll
         for (int k = 0; k < B; ++k)
-            if (w[k] != 0.0f) {
+            if (there[k]) {  // (also with a weight of 0: it must not hide a NaN)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o[e] = fmaf(w[k], v[k][e], o[e]);
             }

@@ -996,3 +996,44 @@ def test_prefill_nan_and_infinite_gates(half, q8, ctx, rows):
     assert torch.equal(got[gt == float("inf")], bare[gt == float("inf")]) and bool((got[gt == -float("inf")] == 0).all())
     same = torch.isfinite(gt)
     assert torch.equal(got[same], want[same])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("ctx,rows,top,at", [(4095, 1, 4000, 700), (4095, 1, 700, 4000), (300, 40, 0, 320), (9000, 70, 8999, 100)])
+def test_prefill_attended_nans_come_out_whatever_their_weight(half, value, ctx, rows, top, at):
+    """One key outweighs the rest by e^200 and more; a value that is not finite still reaches the rows that attend it."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    n = ctx + rows
+    cache = Cache([n], False, 5).fill([n], 6)
+    q, gt = some(rows, 1, kind), some(rows, 2, kind, 1.0)
+    q[:] = q[:1, :1]
+    planes = cache.rows()
+    planes[int(cache.ids[0, top // CH]), 0, :, top % CH] = (8 * q[0, 0]).half()
+    planes[int(cache.ids[0, at // CH]), 1, :, at % CH, 33] = value
+    out = ops.gqa_prefill(q, gt, ints(0, rows), ints(n), rows, n, cache.ptrs(), cache.k_off, cache.v_off).view(rows, H, D)
+    sees = torch.tensor([ctx + r >= at for r in range(rows)], device="cuda")
+    assert not bool(torch.isfinite(out[sees][..., 33]).any())
+    out[..., 33][sees] = 0
+    assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.gpu
+def test_prefill_nan_values_of_infinitely_low_scores_come_out():
+    """A part of which every score is -infinity (f16: 0 times an infinity does not come up) still has its values."""
+    from qwowl35_b200 import ops
+    n = 4096
+    cache = Cache([n], False, 5).fill([n], 6)
+    q = some(1, 1, torch.float16)
+    q[..., 0] = 1.0
+    planes = cache.rows()
+    chunk = int(cache.ids[0, 2])
+    planes[chunk, 0, :, :128, 0] = -float("inf")
+    args = (None, ints(0, 1), ints(n), 1, n, cache.ptrs(), cache.k_off, cache.v_off)
+    assert bool(torch.isfinite(ops.gqa_prefill(q, *args)).all())
+    planes[chunk, 1, :, 77, 33] = float("nan")
+    bad = torch.zeros(H, D, dtype=torch.bool, device="cuda")
+    bad[:, 33] = True
+    assert torch.equal(ops.gqa_prefill(q, *args).view(H, D).isnan(), bad)
