@@ -158,10 +158,11 @@ int qw35_cuda_gqa_decode_noalloc(uint32_t n_seq, const float *q, const float *ga
 // device memory, so the calls can be captured into a CUDA graph and replayed
 // over other lengths within the host's upper bounds.  q, gate and out are
 // [rows][16][256], 16-byte aligned, as is every chunk address; an f32 q and what
-// the cache stands for lie within the f16 range.  A workspace serves one call at
-// a time: calls that may overlap on the GPU (other streams, other graphs) need
-// their own.  The size queries give 0 for sizes that the call refuses or that
-// leave it nothing to do.
+// the cache stands for lie within the f16 range.  Attended positions whose table
+// entry is 0 (a chunk that is missing) count as K and V rows of zeros.  A
+// workspace serves one call at a time: calls that may overlap on the GPU (other
+// streams, other graphs) need their own.  The size queries give 0 for sizes that
+// the call refuses or that leave it nothing to do.
 
 // Appends n_tok tokens to the cache: per-head RMS norm of q and k, rotary
 // positions on dims [0, 64) (NeoX pairs i, i + 32), K and V rows written for table

@@ -770,11 +770,14 @@ __device__ __forceinline__ void attend_exactly(const AttnTileArgs &p, const Tile
     for (int j = s.begin; j < s.end; ++j) {
         const int t = tile_at(s, j);
         const uint64_t base = p.chunk_ptrs[(size_t)s.table * p.max_chunks + t * tk / ACHUNK];
-        for (int pos = t * tk; pos < (t + 1) * tk && base; ++pos) {
+        for (int pos = t * tk; pos < (t + 1) * tk; ++pos) {
             if (pos < s.lo || pos >= hi || (pos >= sk && pos < rs)) continue;
             const size_t row = (size_t)s.kvh * ACHUNK + pos % ACHUNK;
-            auto values = [&](uint64_t plane, float *x) {
-                if constexpr (Q8) {
+            auto values = [&](uint64_t plane, float *x) {  // (zeros of a chunk that is missing, as the tiles have them)
+                if (base == 0) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+                } else if constexpr (Q8) {
                     const uint8_t *blk = reinterpret_cast<const uint8_t *>(plane) + row * kKvQ8Row + 34 * (lane >> 2);
                     const float d = __half2float(*reinterpret_cast<const __half *>(blk));
 #pragma unroll

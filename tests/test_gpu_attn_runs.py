@@ -1037,3 +1037,28 @@ def test_prefill_nan_values_of_infinitely_low_scores_come_out():
     bad = torch.zeros(H, D, dtype=torch.bool, device="cuda")
     bad[:, 33] = True
     assert torch.equal(ops.gqa_prefill(q, *args).view(H, D).isnan(), bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("seqs,n,rows", [(1, 1100, 5), (1, 1100, 1100), (40, 700, 3)])  # joined; pairs; single CTAs
+def test_prefill_missing_chunks_are_zeros(half, q8, seqs, n, rows):
+    """Also in units that a value that is not finite sends to the CUDA cores."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    cache = Cache([n] * seqs, q8, 5).fill([n] * seqs, 6)
+    cache.rows()[cache.ids[:, 1].cuda()] = 0
+    table = cache.ptrs()
+    table[:, 1] = 0
+    q, gt = some(rows * seqs, 1, kind), some(rows * seqs, 2, kind, 1.0)
+    off = ints(*range(0, rows * seqs + 1, rows))
+    kv = [cache.sequence(i, n - 1) for i in range(seqs)]
+    for poisoned in (False, True):
+        if poisoned:
+            for i in range(seqs):
+                poison(cache, i, (n - 1,), float("nan"), planes=(1,))
+        out = ops.gqa_prefill(q, gt, off, ints(*[n] * seqs), rows, n, table, cache.k_off, cache.v_off, kv_q8=q8)
+        ref = [(i * rows + r, *attend(q[i * rows + r], gt[i * rows + r], *kv[i], n - rows + r + 1), n - rows + r + 1)
+               for i in range(0, seqs, 13) for r in sorted({0, 1, rows // 2, rows - 2})]
+        check_rows(out, ref, half, q8)
+        assert not poisoned or not bool(torch.isfinite(out[rows - 1::rows]).all(1).any())
