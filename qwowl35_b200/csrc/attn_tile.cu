@@ -1223,7 +1223,8 @@ TilePlan plan_for(int n_row, int n_run, int max_run, int max_len, int max_own, b
     // to plan, and leave SMs without a part: half the length then, two waves at most.
     const int kv = ceil_div(max_len, kPlanTile), kv_own = ceil_div(max_own, kPlanTile) + 1;
     const long long work = (long long)AKV * ((long long)pl.tiles * kv + (long long)n_row * (1 + kv_own / 2));
-    pl.each = ceil_div(work, (n_run > 1 ? 2 : 1) * kPlanSMs);
+    const long long sms = (n_run > 1 ? 2 : 1) * kPlanSMs;
+    pl.each = (int)std::min<long long>((work + sms - 1) / sms, std::max(kv, kv_own));  // (the quotient can pass 32 bits)
     pl.ns = kv > 0 ? ceil_div(kv, pl.each) : 1;
     pl.own_tiles = n_row;
     pl.ns_own = ceil_div(kv_own, pl.each);

@@ -15,12 +15,16 @@ The sigmoid gate (at most 1) multiplies all of it, with 2^-22 |o| of its own.
 """
 import ctypes as C
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
 
 from qwowl35_b200 import _lib
 
+ROOT = Path(__file__).resolve().parent.parent
 H, KV, D, CH = 16, 4, 256, 256
 Q8ROW = 272
 EPS = 1e-6
@@ -1062,3 +1066,16 @@ def test_prefill_missing_chunks_are_zeros(half, q8, seqs, n, rows):
                for i in range(0, seqs, 13) for r in sorted({0, 1, rows // 2, rows - 2})]
         check_rows(out, ref, half, q8)
         assert not poisoned or not bool(torch.isfinite(out[rows - 1::rows]).all(1).any())
+
+
+# ---- sizes at the limits --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("sizes", [(61731, 51426, 484746496, 505329920), (65535, 1, 1 << 29, 1 << 29), (65535, 65535, 1 << 29, 0),
+                                   (65535, 65535, 1 << 29, 1 << 29)])
+def test_shared_workspace_of_the_largest_sizes(sizes):
+    """More work than 32 bits hold, a share at a time: a part for the prefix and one for the tail.  (In a process of its own: a
+    division by zero would end it.)"""
+    code = "from qwowl35_b200 import _lib; print(_lib.lib().qw35_cuda_gqa_decode_shared_workspace_bytes(*%r))" % (sizes,)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert r.returncode == 0, r.returncode
+    assert int(r.stdout) == sizes[0] * 16 * 2 * (8 + 1024)
