@@ -175,6 +175,7 @@ int qw35_cuda_gqa_decode_noalloc(uint32_t n_seq, const float *q, const float *ga
 // else by axis 0.  A token whose table row or position lies outside
 // [0, n_seq) x [0, 256 max_chunks), or whose table entry is 0, is padding:
 // nothing of it is written.  No two tokens may have the same row and position.
+// A q8_0 block that takes in a NaN or an infinity stands for NaNs.
 int qw35_cuda_attn_append(uint32_t n_tok, const float *qkv, uint32_t qkv_stride, const float *q_norm_w,
                           const float *k_norm_w, const float *rope_freq, const int32_t *rope_pos, uint32_t n_axes,
                           const int32_t *sections, int interleaved, const int32_t *tok_seq, const int32_t *tok_pos,

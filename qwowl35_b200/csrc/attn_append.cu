@@ -97,8 +97,8 @@ __device__ __forceinline__ void write_row(const AttnAppendArgs &p, int tok, int 
     const size_t at = (size_t)(head - AH) * ACHUNK + (pos % ACHUNK);
     if constexpr (Q8) {  // lanes 4b..4b+3 hold block b
         uint8_t *blk = reinterpret_cast<uint8_t *>(base) + at * kKvQ8Row + 34 * (lane >> 2);
-        q8_block_store(v, blk + p.k_off, lane);
-        q8_block_store(g, blk + p.v_off, lane);
+        q8_block_store<true>(v, blk + p.k_off, lane);  // (a NaN stays one, as in f16 planes)
+        q8_block_store<true>(g, blk + p.v_off, lane);
     } else {
         store8(reinterpret_cast<__half *>(base + p.k_off) + at * AHD + d0, v);
         store8(reinterpret_cast<__half *>(base + p.v_off) + at * AHD + d0, g);

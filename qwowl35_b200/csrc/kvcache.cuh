@@ -17,12 +17,21 @@ constexpr int QFULL = AH * AHD * 2;  // q | gate per head
 // d = amax / 127 in fp32, codes round(x * (1 / d)) (half away from zero)
 // clamped to +-127 with the fp32 d, the block stores half(d).  `blk` points at
 // the block's 34 bytes {f16 d; int8 qs[32]}; every lane of the warp calls this.
+// fmaxf passes over NaNs, as the reference's maximum does: they become codes of 0
+// in a block of the others.  NANS: a block that has one gets a NaN d instead.
+template <bool NANS = false>
 __device__ __forceinline__ void q8_block_store(const float *x, uint8_t *blk, int lane) {
+    auto larger = [](float a, float b) {
+        if constexpr (!NANS) return fmaxf(a, b);
+        float y;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+        return y;
+    };
     float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    for (int i = 0; i < 8; ++i) amax = larger(amax, fabsf(x[i]));
+    amax = larger(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = larger(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const float d = amax / 127.0f;
     const float id = d != 0.0f ? 1.0f / d : 0.0f;
     uint32_t packed[2] = {0u, 0u};

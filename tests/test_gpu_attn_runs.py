@@ -1079,3 +1079,37 @@ def test_shared_workspace_of_the_largest_sizes(sizes):
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
     assert r.returncode == 0, r.returncode
     assert int(r.stdout) == sizes[0] * 16 * 2 * (8 + 1024)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("n", [5, 1000])
+def test_append_nans_come_out(half, q8, n):
+    """A NaN or an infinity of a token's q, gate, k or v is one in what is written of it (q8_0: in its block), and nowhere else."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    g = torch.Generator("cuda").manual_seed(n)
+    qkv = torch.randn(n, 10240, device="cuda", generator=g)
+    w, pos = torch.ones(256, device="cuda"), torch.arange(n, device="cuda").int()
+    nan, inf = float("nan"), float("inf")
+    qkv[1, 3 * 512 + 100], qkv[2, 5 * 512 + 256 + 7] = nan, nan                          # q head 3, gate 5
+    qkv[1, 8192 + 256 + 200], qkv[3, 8192 + 1024 + 512 + 77] = nan, nan                  # k head 1, v head 2
+    qkv[2, 8192 + 768 + 200], qkv[4, 8192 + 1024 + 30], qkv[4, 8192 + 1024 + 255] = inf, inf, -inf  # k head 3, v head 0
+    cache = Cache([n], q8, 3).fill([n], 4)
+    q, gate = ops.attn_append(qkv, w, w, FREQ.cuda(), pos[None].contiguous(), (32,), torch.zeros_like(pos), pos, cache.ptrs(), cache.k_off,
+                              cache.v_off, dtype=kind, kv_q8=q8)
+    bad = torch.zeros(n, H, D, dtype=torch.bool, device="cuda")
+    bad[1, 3] = True
+    assert torch.equal(~torch.isfinite(q), bad)
+    bad[:] = False
+    bad[2, 5, 7] = True
+    assert torch.equal(~torch.isfinite(gate), bad)
+    k, v = cache.sequence(0, n)
+    bad = torch.zeros(2, KV, n, D, dtype=torch.bool, device="cuda")
+    wide = slice(192, 224) if q8 else slice(200, 201)
+    bad[0, 1, 1] = True
+    bad[0, 3, 2, wide] = True
+    bad[1, 2, 3, slice(64, 96) if q8 else slice(77, 78)] = True
+    bad[1, 0, 4, slice(0, 32) if q8 else slice(30, 31)] = True
+    bad[1, 0, 4, slice(224, 256) if q8 else slice(255, 256)] = True
+    assert torch.equal(~torch.isfinite(torch.stack([k, v])), bad)
