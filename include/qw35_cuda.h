@@ -187,10 +187,11 @@ int qw35_cuda_attn_append(uint32_t n_tok, const float *qkv, uint32_t qkv_stride,
 // last tokens of sequence i (table row i), whose context length with them is
 // seq_len[i]; the run's row t attends positions [0, seq_len[i] - run length + t],
 // cut by window and sink as in qw35_cuda_gqa_decode.  n_row is the number of rows
-// of q; rows outside every run are left as they were.  max_run and max_len are
-// upper bounds of a run's rows and of seq_len.  What a row does not attend does
-// not reach it, infinities and NaNs included; what lies behind seq_len[i] is not
-// looked at.
+// of q; rows outside every run are left as they were.  max_run (1 to n_row) and
+// max_len (1 to 256 max_chunks) are upper bounds of a run's rows and of seq_len:
+// rows beyond max_run may be left out, lengths beyond max_len only divide the
+// work badly.  What a row does not attend does not reach it, infinities and NaNs
+// included; what lies behind seq_len[i] is not looked at.
 uint64_t qw35_cuda_gqa_prefill_workspace_bytes(uint32_t n_row, uint32_t n_run, uint32_t max_run, uint32_t max_len);
 int qw35_cuda_gqa_prefill(uint32_t n_row, const void *q, const void *gate, uint32_t dtype, uint32_t n_run,
                           const int32_t *run_off, const int32_t *seq_len, uint32_t max_run, uint32_t max_len,

@@ -392,7 +392,7 @@ int qw35_cuda_gqa_prefill(uint32_t n_row, const void *q, const void *gate, uint3
     if (max_run == 0 || max_run > n_row || max_len == 0 || !tile_sizes_ok(n_row, n_run, max_len) ||
         !tile_args(a, n_row, q, gate, dtype, n_run, run_off, seq_len, max_len, chunk_ptrs, max_chunks, k_off, v_off,
                    kv_type, window, sink, out, workspace, workspace_bytes)) {
-        set_err(err, err_len, "invalid prefill attention arguments%s", "");
+        set_err(err, err_len, "invalid prefill attention arguments%s", " (max_run is 1 to n_row, max_len 1 to 256 max_chunks)");
         return 0;
     }
     if (workspace_bytes < qw35_cuda_gqa_prefill_workspace_bytes(n_row, n_run, max_run, max_len)) {
@@ -424,7 +424,7 @@ int qw35_cuda_gqa_decode_shared(uint32_t n_seq, const void *q, const void *gate,
     if (!shared_len || longest == 0 || n_seq > 65535 || !tile_sizes_ok(n_seq, n_group, longest) ||
         !tile_args(a, n_seq, q, gate, dtype, n_group, group_off, seq_len, longest, chunk_ptrs, max_chunks, k_off, v_off,
                    kv_type, window, sink, out, workspace, workspace_bytes)) {
-        set_err(err, err_len, "invalid shared-prefix attention arguments%s", "");
+        set_err(err, err_len, "invalid shared-prefix attention arguments%s", " (max_shared and max_own are at most 256 max_chunks, one of them above 0)");
         return 0;
     }
     if (workspace_bytes < qw35_cuda_gqa_decode_shared_workspace_bytes(n_seq, n_group, max_shared, max_own)) {

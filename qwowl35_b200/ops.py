@@ -257,7 +257,7 @@ def attn_append(qkv, q_norm_w, k_norm_w, rope_freq, rope_pos, sections, tok_seq,
 
 
 def gqa_prefill_workspace(n_row: int, n_run: int, max_run: int, max_len: int, device="cuda"):
-    n = int(lib().qw35_cuda_gqa_prefill_workspace_bytes(n_row, n_run, max_run, max_len))
+    n = int(lib().qw35_cuda_gqa_prefill_workspace_bytes(n_row, n_run, min(max_run, n_row), max_len))
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
@@ -266,10 +266,11 @@ def gqa_prefill(q, gate, run_off, seq_len, max_run, max_len, chunk_ptrs, k_off, 
     """Causal attention of token runs over the cache that already holds them; [n, 4096] in q's type.
 
     run_off [runs + 1], seq_len [runs] int32: rows run_off[i]..run_off[i+1] of q are the last tokens of sequence i.
-    max_run, max_len: upper bounds of the runs' rows and of seq_len.
+    max_run, max_len: upper bounds of the runs' rows and of seq_len, max_len within the table's 256 positions a chunk.
     """
     dev, dtype = _device_of(q), q.dtype
     n, runs, table = q.shape[0], seq_len.numel(), chunk_ptrs.shape
+    max_run = min(max_run, n)  # (the entry point refuses bounds that cannot be reached)
     if table[0] < runs:
         raise ValueError("chunk_ptrs needs a row for every run")
     half, L = _head_dtype(dtype), lib()

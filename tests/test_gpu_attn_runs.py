@@ -1113,3 +1113,15 @@ def test_append_nans_come_out(half, q8, n):
     bad[1, 0, 4, slice(0, 32) if q8 else slice(30, 31)] = True
     bad[1, 0, 4, slice(224, 256) if q8 else slice(255, 256)] = True
     assert torch.equal(~torch.isfinite(torch.stack([k, v])), bad)
+
+
+@pytest.mark.gpu
+def test_prefill_bound_of_rows_may_exceed_them():
+    from qwowl35_b200 import ops
+    cache = Cache([300], False, 5).fill([300], 6)
+    q, gt = some(40, 1, torch.float16), some(40, 2, torch.float16)
+    at = (cache.ptrs(), cache.k_off, cache.v_off)
+    want = ops.gqa_prefill(q, gt, ints(0, 40), ints(300), 40, 300, *at)
+    ws = ops.gqa_prefill_workspace(40, 1, 64, 300)
+    for kw in ({}, {"ws": ws}):
+        assert torch.equal(ops.gqa_prefill(q, gt, ints(0, 40), ints(300), 64, 300, *at, **kw), want)
