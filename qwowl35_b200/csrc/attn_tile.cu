@@ -32,7 +32,8 @@
 //
 // The running maximum is lazy: O is rescaled only when a row's maximum grows by
 // more than 2^8 over the one in use, so P reaches at most 2^15 (its 2^7 offset
-// keeps small probabilities out of f16's denormals).  Sums and O are f32.
+// keeps small probabilities out of f16's denormals).  Sums and O are f32; O leaves
+// TMEM in pieces (kAwayF32), as the tensor cores truncate what they add.
 //
 // Work is split along the positions where there are few row tiles; the parts'
 // (m, l, O) go through the workspace and attn_join_kernel merges them.
@@ -58,6 +59,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kShift = 7.0f, kSlack = 8.0f;  // log2: offset of P, growth of the maximum before O is rescaled
 constexpr float kNoScore = -3.0e38f;  // the maximum that a part leaves which has values but no finite score (an empty one: -infinity)
 
+// Positions that one O in TMEM sums up before the softmax warps put it away, adding it, rounded to nearest, to the row's sum
+// in the workspace, and the next product starts anew.  The tensor cores' adder truncates, which costs O about 2e-8 a step
+// of 16 positions and operand half.  f32 in one chain: 2.1e-5 (2-norm) after 8,192 positions, 8.7e-5 after 32,768 (q8_0
+// 17e-5), in pieces 6e-6 (10e-6), for which a prompt of 4,096 takes 317 us instead of 296, of 8,192 853 instead of 779, of
+// 32,768 13.0 ms instead of 12.4.  f16 has half the steps and 24e-5 of its own rounding, so its pieces are longer.  Parts no
+// longer than a piece take a kernel that cannot put away (AWAY false): f16 8192 tokens 435 us against 443 with one that can.
+constexpr int kAwayF32 = 2048, kAwayF16 = 65536;
+
 template <bool HL, bool Q8, bool PAIR>
 struct TileGeo {
     static constexpr int CTAS = PAIR ? 2 : 1;
@@ -81,6 +90,7 @@ struct TileGeo {
     static constexpr int PARTS = HL && Q8 ? 2 : 1;       // stages of a tile: values, or their hi and lo halves
     static constexpr uint32_t RING = NST * STAGE, SMEM = QB + RING;
     static constexpr uint32_t S0 = 256;                  // TMEM columns: O, then the S buffers, then (LO_TMEM) Q's lo half
+    static constexpr int AWAY = (HL ? kAwayF32 : kAwayF16) / TK;  // tiles after which O is put away
     // a lo half bound for TMEM passes through the last 64 KB of the ring
     static constexpr int FREE_AT_START = LO_TMEM ? (int)((RING - QBYTES) / STAGE) : NST;
 };
@@ -92,6 +102,7 @@ struct TilePlan {
     int own_tiles;  // shared prefixes: sequences with a tail of their own, else 0
     int ns_own;     // position splits of a tail (upper bound)
     int each;       // kPlanTile tiles of a split
+    int room;       // the workspace has room for O that is put away
 };
 
 constexpr uint32_t kQlo = 384;  // TMEM columns of the lo half of Q
@@ -246,18 +257,13 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo = pack2(a - f.x, b - f.y);
 }
 
-// 1 / (1 + e^-x) to 2^-20 (ex2 and the quotient 2^-22 each; sigmoid_f's exact division and exponential cost an epilogue
-// 4 us); below the smallest normal number 0, and NaN for NaN.  t = -x log2 e is rounded, by up to 2^-18 for gates of
-// -80, so what it lost (r, with the rest of log2 e) enters as a factor 1 + r ln 2.  The ends, beyond which f32 has 0 or
-// 1, keep e within what __fdividef divides by (2^126) and infinities out of r.
+// 1 / (1 + e^-x): f32 to 2^-21 (expf 2 units, quotient 2^-22; sigmoid_f's exact division cost an epilogue 4 us), f16, by
+// ex2 of a rounded argument, to 2^-18 at gates of -80.  0 below the smallest normal number (__fdividef by 2^126 and more),
+// NaN for NaN: no clamp, which would take the bound for a NaN.
+template <typename T>
 __device__ __forceinline__ float sigmoid_fast(float x) {
-    float z;
-    asm("{\n\t.reg .f32 a;\n\tmax.NaN.f32 a, %1, %2;\n\tmin.NaN.f32 %0, a, %3;\n\t}" : "=f"(z) : "f"(x), "f"(-87.33654f), "f"(88.0f));
-    const float t = -z * kLog2e;
-    const float r = fmaf(-z, 1.92596303e-8f, fmaf(-z, kLog2e, -t));
-    const float e = ex2(t);
-    const float y = __fdividef(1.0f, 1.0f + fmaf(e, r * 0.693147181f, e));
-    return x < -87.33654f ? 0.0f : y;
+    const float e = std::is_same<T, float>::value ? expf(-x) : ex2(-x * kLog2e);
+    return __fdividef(1.0f, 1.0f + e);
 }
 
 // 8 consecutive values of a row, 16-byte aligned
@@ -281,6 +287,9 @@ __device__ __forceinline__ void put8(float *p, const float *v) {
 }
 __device__ __forceinline__ void put8(__half *p, const float *v) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+}
+__device__ __forceinline__ void red_add4(float4 *p, const float *v) {
+    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1,%2,%3,%4};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]) : "memory");
 }
 __device__ __forceinline__ int warp_min_i(int v) { return __reduce_min_sync(0xffffffffu, v); }
 __device__ __forceinline__ int warp_max_i(int v) { return __reduce_max_sync(0xffffffffu, v); }
@@ -648,7 +657,7 @@ struct Loader {
 };
 
 // ---- products (one warp; of a pair, the leader's) ------------------------------------
-template <bool HL, bool Q8, bool PAIR>
+template <bool HL, bool Q8, bool PAIR, bool AWAY>
 struct Products {
     using G = TileGeo<HL, Q8, PAIR>;
     TileShared &s;
@@ -703,12 +712,13 @@ struct Products {
         constexpr uint32_t idesc = idesc_f16_f32(TM_ROWS * G::CTAS, AHD) | (1u << 16);  // B MN-major
         const uint32_t v0 = stage(0), v1 = G::PARTS > 1 ? stage(1) : v0;
         const uint64_t vd0 = desc_v(v0, G::TK * 128u), vd1 = desc_v(v1, G::TK * 128u);
+        const bool on = AWAY ? j % G::AWAY > 0 : j > 0;  // onto what O holds
         if (elect_one()) {
 #pragma unroll
             for (int i = 0; i < G::TK / 16; ++i) {  // 16 positions: 2048 bytes on
-                if constexpr (HL) mma_ts<PAIR>(tmem, pa + G::TK / 2 + i * 8, vd0 + i * 128, idesc, j > 0 || i > 0);
+                if constexpr (HL) mma_ts<PAIR>(tmem, pa + G::TK / 2 + i * 8, vd0 + i * 128, idesc, on || i > 0);
                 if constexpr (HL && Q8) mma_ts<PAIR>(tmem, pa + i * 8, vd1 + i * 128, idesc, 1);
-                mma_ts<PAIR>(tmem, pa + i * 8, vd0 + i * 128, idesc, HL || j > 0 || i > 0);
+                mma_ts<PAIR>(tmem, pa + i * 8, vd0 + i * 128, idesc, HL || on || i > 0);
             }
             commit<PAIR>(&s.pv_done);
         }
@@ -804,7 +814,7 @@ __device__ __forceinline__ void attend_exactly(const AttnTileArgs &p, const Tile
 }
 
 // ---- the kernel ---------------------------------------------------------------------
-template <bool HL, bool Q8, bool PAIR>
+template <bool HL, bool Q8, bool PAIR, bool AWAY>
 __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_kernel(AttnTileArgs p, TilePlan pl) {
     using G = TileGeo<HL, Q8, PAIR>;
     using T = typename std::conditional<HL, float, __half>::type;
@@ -861,7 +871,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
     } else if (warp >= MMA_WARP) {
         set_regs<G::SPLIT, G::REST_REGS, false>();
         if (warp == MMA_WARP && rank == 0) {
-            Products<HL, Q8, PAIR> mm{s, sbase, sbase + G::QB, tmem};
+            Products<HL, Q8, PAIR, AWAY> mm{s, sbase, sbase + G::QB, tmem};
             mm.run();
         } else if (warp == MMA_WARP + 1 && lane == 0) {
             relay<HL, Q8, PAIR>(s, rank);
@@ -950,7 +960,59 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
         const int hi = real ? s.hi[tok] : 0x7fffffff, sk = real ? s.sk[tok] : 0, rs = real ? s.rs[tok] : 0;
         float m = -INFINITY, l = 0.0f;  // maximum in use; sum of this half's columns
         constexpr int CW = G::TK / 2, NB = CW / 32;
-        for (int j = 0; j < n; ++j) {
+        const int parts = pl.ns + pl.ns_own;
+        float *acc = reinterpret_cast<float *>(static_cast<float2 *>(p.ws) + (size_t)p.n_row * AH * parts);
+        float ma = -INFINITY;  // maximum in use when O was put away
+        // Where this lane's 16 dims (16 b on) of O go, in four pieces: along its row or, for a full warp, in two heads' halves of
+        // one of the warp's tokens, 512 bytes a store (a row a lane is 32 lines a store).  (Worked out where it is used: what
+        // the tile loop would have to keep of it is spilled.)
+        struct Place {
+            float *at;
+            int hop, half;
+            __device__ __forceinline__ float4 *piece(int i) const { return reinterpret_cast<float4 *>(at + i / 2 * hop + i % 2 * half); }
+        };
+        auto place = [&](int b) {
+            int r = row;
+            asm volatile("" : "+r"(r));
+            const int q = r & ~31, part = s.part;
+            const bool full = q + 32 <= s.nrow * AGRP;
+            const size_t h = head_row(full ? q + b / 2 * AGRP + b % 2 * 2 : r) * parts + part;
+            return Place{acc + h * AHD + (full ? (r & 31) * 4 : b * 16), full ? parts * AHD : 8, full ? AHD / 2 : 4};
+        };
+        auto grown = [&]() { return ma == -INFINITY ? 1.0f : ex2((ma - m) * c); };  // (without a score so far: 0, or NaN and to stay so)
+        // O onto what was put away by additions in L2, which nothing waits for; no other thread has these values, so their
+        // order is this one's.  Where a maximum grew since the last time, what is there takes its units first.
+        auto put_away = [&](bool first) {
+            const float f = first || !real ? 1.0f : grown();
+            if (__any_sync(0xffffffffu, f != 1.0f)) {
+#pragma unroll 1
+                for (int b = grp * 8; b < grp * 8 + 8 && real; ++b) {
+                    const Place at = place(b);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 x = __ldcg(at.piece(i));
+                        __stcg(at.piece(i), make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+                    }
+                }
+                __syncwarp();
+            }
+#pragma unroll 1
+            for (int b = grp * 8; b < grp * 8 + 8; ++b) {
+                const Place to = place(b);
+                float o[16];
+                tmem_ld16(tmem + lanes + b * 16, o);
+                if (real) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (!first) red_add4(to.piece(i), o + 4 * i);
+                        else __stcg(to.piece(i), make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+                    }
+                }
+                __syncwarp();
+            }
+            ma = m;
+        };
+        auto tile = [&](int j) {
             const uint32_t sb = tmem + lanes + G::S0 + (j & 1) * G::TK;
             tw(&s.s_full[j & 1], (uint32_t)(j >> 1) & 1u, s, 32u);
             tc_fence_after();
@@ -1028,11 +1090,21 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 if (PAIR && rank) arrive_leader<false>(&s.p_full[j & 1]);
                 else mbar_arrive(&s.p_full[j & 1]);
             }
+        };
+        for (int j = 0, stop = 0; j < n;) {
+            stop = AWAY ? min(n, stop + G::AWAY) : n;
+            for (; j < stop; ++j) tile(j);
+            if (AWAY && j < n && busy) {
+                tw(&s.s_full[j & 1], (uint32_t)(j >> 1) & 1u, s, 32u);  // (so the product of j - 2 has ended: one parity bit tells j - 1)
+                tw(&s.pv_done, (uint32_t)(j - 1) & 1u, s, 64u);
+                tc_fence_after();
+                put_away(j == G::AWAY);
+            }
         }
 
         // O goes, scaled, to rows of the (free) ring and from there out coalesced, a warp per row; the gates of the
         // first rows are fetched before the last product ends
-        const int parts = pl.ns + pl.ns_own, rows = s.nrow * AGRP;
+        const int rows = s.nrow * AGRP;
         const bool join = parts > 1;
         constexpr int EB = HL ? 4 : 8;  // rows a batch
         uint4 gates[EB][HL ? 2 : 1];
@@ -1074,23 +1146,40 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
         } else if (busy) {
             const float inv = join ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
             if (n > 0) {
+                if (AWAY && n > G::AWAY) {
+#pragma unroll 1
+                    for (int b = grp * 8; b < grp * 8 + 8; ++b) {
+                        const Place from = place(b);
+                        const float f = grown();
+                        float o[16];
+                        float4 x[4];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    uint32_t o[32];
-                    tmem_ld32_async(tmem + lanes + grp * 128 + b * 32, o);
-                    tmem_ld_wait();
+                        for (int i = 0; i < 4; ++i)
+                            if (real) x[i] = __ldcg(from.piece(i));
+                        __syncwarp();
+                        tmem_ld16(tmem + lanes + b * 16, o);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4 *>(buf + row * BROW + grp * 128 + b * 32 + i) =
-                            make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv,
-                                        __uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<float4 *>(buf + row * BROW + b * 16 + 4 * i) =
+                                make_float4(fmaf(x[i].x, f, o[4 * i]) * inv, fmaf(x[i].y, f, o[4 * i + 1]) * inv,
+                                            fmaf(x[i].z, f, o[4 * i + 2]) * inv, fmaf(x[i].w, f, o[4 * i + 3]) * inv);
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        float o[32];
+                        tmem_ld32(tmem + lanes + grp * 128 + b * 32, o);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<float4 *>(buf + row * BROW + grp * 128 + b * 32 + i) =
+                                make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                    }
                 }
             }
             if (join && real && grp == 0)
                 static_cast<float2 *>(p.ws)[head_row(row) * parts + s.part] = make_float2(m == -INFINITY ? kNoScore : fmaf(m, c, -kShift), l);
         }
         named_sync(9, SOFT_WARPS * 32);
-        float *acc = reinterpret_cast<float *>(static_cast<float2 *>(p.ws) + (size_t)p.n_row * AH * parts);
         for (int r0 = warp; r0 < rows; r0 += SOFT_WARPS * EB) {
             if (r0 != warp) fetch_gates(r0);
 #pragma unroll
@@ -1108,7 +1197,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                     float gv[8];
                     get8(reinterpret_cast<const T *>(&gates[i][0]), gv);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] *= sigmoid_fast(gv[e]);
+                    for (int e = 0; e < 8; ++e) y[e] *= sigmoid_fast<T>(gv[e]);
                 }
                 put8(static_cast<T *>(p.out) + g * AHD + lane * 8, y);
             }
@@ -1185,7 +1274,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_join_kernel(AttnTileArgs
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         o[e] *= inv;
-        if (p.gate) o[e] *= sigmoid_fast(gv[e]);
+        if (p.gate) o[e] *= sigmoid_fast<T>(gv[e]);
     }
     put8(static_cast<T *>(p.out) + g * AHD + lane * 8, o);
 }
@@ -1216,6 +1305,7 @@ TilePlan plan_for(int n_row, int n_run, int max_run, int max_len, int max_own, b
         if (pl.ns > kv) pl.ns = kv;
         pl.each = ceil_div(kv, pl.ns);
         pl.ns = ceil_div(kv, pl.each);
+        pl.room = pl.ns > 1 || max_len > kAwayF32;
         return pl;
     }
     // Shared prefixes.  Parts of one length: what one wave of CTAs would get each, a tail counting as its setup (a
@@ -1228,18 +1318,19 @@ TilePlan plan_for(int n_row, int n_run, int max_run, int max_len, int max_own, b
     pl.ns = kv > 0 ? ceil_div(kv, pl.each) : 1;
     pl.own_tiles = n_row;
     pl.ns_own = ceil_div(kv_own, pl.each);
+    pl.room = 1;  // (a prefix and a tail: always joined)
     return pl;
 }
 
 size_t parts_bytes(int n_row, const TilePlan &pl) {
-    const int parts = pl.ns + pl.ns_own;
-    return parts > 1 ? (size_t)n_row * AH * parts * (sizeof(float2) + AHD * sizeof(float)) : 256;
+    const int parts = pl.ns + pl.ns_own;  // (f16 calls put away later than this allows for: the query has no type)
+    return pl.room ? (size_t)n_row * AH * parts * (sizeof(float2) + AHD * sizeof(float)) : 256;
 }
 
-template <bool HL, bool Q8, bool PAIR>
-cudaError_t launch_tile(const AttnTileArgs &a, const TilePlan &pl, cudaStream_t st) {
+template <bool HL, bool Q8, bool PAIR, bool AWAY>
+cudaError_t launch_one(const AttnTileArgs &a, const TilePlan &pl, cudaStream_t st) {
     using G = TileGeo<HL, Q8, PAIR>;
-    auto kern = attn_tile_kernel<HL, Q8, PAIR>;
+    auto kern = attn_tile_kernel<HL, Q8, PAIR, AWAY>;
     constexpr int smem = (int)(G::SMEM + sizeof(TileShared));
     static_assert(smem <= 227 * 1024, "stages and Q fit one SM");
     static_assert(G::NST <= kMaxStages, "a barrier for every stage");
@@ -1259,6 +1350,12 @@ cudaError_t launch_tile(const AttnTileArgs &a, const TilePlan &pl, cudaStream_t 
     cfg.attrs = at;
     cfg.numAttrs = PAIR ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kern, a, pl);
+}
+
+template <bool HL, bool Q8, bool PAIR>
+cudaError_t launch_tile(const AttnTileArgs &a, const TilePlan &pl, cudaStream_t st) {
+    const bool away = pl.room && (long long)pl.each * kPlanTile > (HL ? kAwayF32 : kAwayF16);
+    return away ? launch_one<HL, Q8, PAIR, true>(a, pl, st) : launch_one<HL, Q8, PAIR, false>(a, pl, st);
 }
 
 template <bool PAIR>

@@ -1125,3 +1125,95 @@ def test_prefill_bound_of_rows_may_exceed_them():
     ws = ops.gqa_prefill_workspace(40, 1, 64, 300)
     for kw in ({}, {"ws": ws}):
         assert torch.equal(ops.gqa_prefill(q, gt, ints(0, 40), ints(300), 64, 300, *at, **kw), want)
+
+
+# ---- long contexts --------------------------------------------------------------------------------------
+
+LONG = [(False, False, 32768), (False, True, 32768), (True, False, 140000), (True, True, 140000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8,n", LONG)
+@pytest.mark.parametrize("runs,rows", [(1, 1300), (40, 3), (16, 1)])  # pairs and single CTAs in one piece; joined from two
+def test_prefill_over_long_contexts_stays_exact(half, q8, n, runs, rows):
+    """In the 2-norm of a head's row.  O sums at most 2,048 positions in a chain of truncated steps (2^-23 each, 16 positions and
+    operand half; q8_0 three), f16 65,536 in steps of half; the rest as over short contexts."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    cache = Cache([n], q8, 5).fill([n], 6)
+    q, gt = some(runs * rows, 1, kind), some(runs * rows, 2, kind, 1.0)
+    table = cache.ptrs().expand(runs, -1).contiguous()
+    for poisoned in (False, True):
+        if poisoned:  # (the last row of each run attends it)
+            poison(cache, 0, (n - 1,), float("nan"), planes=(1,))
+        out = ops.gqa_prefill(q, gt, ints(*range(0, runs * rows + 1, rows)), ints(*[n] * runs), rows, n, table, cache.k_off, cache.v_off,
+                              kv_q8=q8)
+        k, v = cache.sequence(0, n)
+        chain = 65536 / 16 * 2.0 ** -23 + (2.0 ** -10 if q8 else 2.0 ** -11) if half else 2048 / 16 * (3 if q8 else 2) * 2.0 ** -23
+        for r in sorted({0, rows // 2, max(rows - 2, 0), (runs // 2) * rows}):
+            if poisoned and r % rows == rows - 1:
+                assert not bool(torch.isfinite(out[r]).all())
+                continue
+            see = n - rows + r % rows + 1
+            o = attend(q[r], gt[r], k[:, :see], v[:, :see], see)[0]
+            err = float(((out[r].double().view(H, D) - o).norm(dim=-1) / o.norm(dim=-1)).max())
+            assert err <= 2.0 ** -18 + chain, (r, err)
+    assert _lib.lib().qw35_cuda_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8,n", LONG)
+@pytest.mark.parametrize("up", [True, False])
+@pytest.mark.parametrize("runs,rows", [(1, 1300), (40, 3)])
+def test_prefill_scores_that_climb_and_fall_over_a_long_context(half, q8, n, up, runs, rows):
+    """The maximum grows from tile to tile, over what was put away too; or every later position counts for less."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    cache = Cache([n], q8, 5).fill([n], 6, 0.25)
+    q, gt = some(runs * rows, 1, kind, 0.3), some(runs * rows, 2, kind, 1.0)
+    q[..., 7] = 3.0
+    ramp = torch.arange(n, device="cuda", dtype=torch.float32) / n * (1.0 if up else -1.0)
+    rows_k = cache.rows()
+    for c in range(-(-n // CH)):
+        part, m = rows_k[int(cache.ids[0, c])], min(CH, n - c * CH)
+        if q8:  # (block 0: dim 7's code at its largest, d so that d * 127 is the ramp's value)
+            part[0, :, :m, 0, 2:] = 0
+            part[0, :, :m, 0, 2 + 7] = 127
+            d = (ramp[c * CH:c * CH + m] * 200 / 127).half()
+            part[0, :, :m, 0, :2] = d.view(torch.uint8).view(m, 2)
+        else:
+            part[0, :, :m, 7] = (ramp[c * CH:c * CH + m] * 200).half()
+    table = cache.ptrs().expand(runs, -1).contiguous()
+    out = ops.gqa_prefill(q, gt, ints(*range(0, runs * rows + 1, rows)), ints(*[n] * runs), rows, n, table, cache.k_off, cache.v_off, kv_q8=q8)
+    k, v = cache.sequence(0, n)
+    ref = []
+    for r in sorted({0, rows // 2, rows - 1, (runs // 2) * rows}):
+        see = n - rows + r % rows + 1
+        ref.append((r, *attend(q[r], gt[r], k[:, :see], v[:, :see], see), see))
+    check_rows(out, ref, half, q8)
+    assert _lib.lib().qw35_cuda_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8", [(False, False), (False, True), (True, False)])
+@pytest.mark.parametrize("window,sink", [(0, 0), (1000, 5)])
+def test_shared_over_long_prefixes(half, q8, window, sink):
+    """Forty pairs of sequences behind one long prefix: parts long enough to put O away; with a window, a sequence that ends early
+    attends nothing of most of its part."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    shared, groups = 30000, 40
+    cache = Cache([shared + 100, shared + 100], q8, 5).fill([shared + 100] * 2, 6)
+    cache.ids[1, :shared // CH] = cache.ids[0, :shared // CH]
+    planes = cache.rows()
+    planes[int(cache.ids[1, shared // CH])][:, :, :shared % CH] = planes[int(cache.ids[0, shared // CH])][:, :, :shared % CH]
+    lens = [5000, shared + 77] * groups
+    q, gt = some(2 * groups, 1, kind), some(2 * groups, 2, kind, 1.0)
+    out = ops.gqa_decode_shared(q, gt, ints(*lens), ints(*range(0, 2 * groups + 1, 2)), ints(*[shared] * groups), shared, 100,
+                                cache.ptrs().repeat(groups, 1), cache.k_off, cache.v_off, window=window, sink=sink, kv_q8=q8)
+    ref = []
+    for r in (0, 1, 40, 79):
+        k, v = cache.sequence(r % 2, lens[r])
+        ref.append((r, *attend(q[r], gt[r], k, v, lens[r], window, sink), lens[r]))
+    check_rows(out, ref, half, q8)
+    assert _lib.lib().qw35_cuda_device_error() == 0
