@@ -1217,3 +1217,91 @@ def test_shared_over_long_prefixes(half, q8, window, sink):
         ref.append((r, *attend(q[r], gt[r], k, v, lens[r], window, sink), lens[r]))
     check_rows(out, ref, half, q8)
     assert _lib.lib().qw35_cuda_device_error() == 0
+
+
+# ---- more of runs: pairs, repeats, precision ---------------------------------------------------------------
+
+def wants_pairs(ctx, rows):
+    """The rule by which one run goes to CTA pairs: more than a tile of rows, and two row tiles x 128 positions an SM."""
+    return rows > 32 and ((rows - 1) // 32 + 1) * KV * -(-(ctx + rows) // 128) > 2 * 148
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("half,q8", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("ctx,rows,window,sink", [(2000, 200, 0, 0), (9000, 70, 0, 0), (3000, 300, 120, 3)])
+@pytest.mark.parametrize("dim", [5, 250])
+def test_prefill_on_pairs_keeps_what_a_row_does_not_attend_from_it(value, half, q8, ctx, rows, window, sink, dim):
+    """A value in either half of the dims, at positions that some rows of either CTA of a pair do not attend."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    assert wants_pairs(ctx, rows)
+    n = ctx + rows
+    q, gt = some(rows, 1, kind), some(rows, 2, kind, 1.0)
+    for at in (ctx + 10, ctx + 45, ctx + rows - 1):
+        cache = Cache([n], q8, 5).fill([n], 6)
+        part = cache.rows()[int(cache.ids[0, at // CH]), 1, :, at % CH]
+        if q8:
+            part[:, dim // 32, :2] = torch.tensor([value], dtype=torch.float16).view(torch.uint8).cuda()
+        else:
+            part[:, dim] = value
+        out = ops.gqa_prefill(q, gt, ints(0, rows), ints(n), rows, n, cache.ptrs(), cache.k_off, cache.v_off, window=window, sink=sink, kv_q8=q8)
+        k, v = cache.sequence(0, n)
+        wide = ~torch.isfinite(v[0, at])
+        k, v = k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0)
+        for r in range(0, rows):
+            length = ctx + r + 1
+            hit = at < length and (window <= 0 or at >= length - window)
+            y = out[r].view(H, D)
+            assert torch.equal(~torch.isfinite(y), (wide & hit).expand(H, D)), (r, at)
+            if r % 9 == 0 or abs(r - (at - ctx)) < 2:
+                o, a, s = attend(q[r], gt[r], k, v, length, window, sink)
+                err = ((y.double() - o).abs() / bound(o, a, s, length, half, q8))[:, ~wide]
+                assert float(err.max()) <= 1.0, (r, at)
+    assert _lib.lib().qw35_cuda_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("half,q8", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("ctx,rows", [(4095, 1), (2000, 200), (0, 1500), (0, 5000)])
+def test_prefill_repeats_itself(half, q8, ctx, rows):
+    """The same bits every time; 5,000 positions leave TMEM in pieces (f32)."""
+    from qwowl35_b200 import ops
+    kind = torch.float16 if half else torch.float32
+    n = ctx + rows
+    cache = Cache([n], q8, 5).fill([n], 6)
+    q, gt = some(rows, 1, kind), some(rows, 2, kind, 1.0)
+    args = (q, gt, ints(0, rows), ints(n), rows, n, cache.ptrs(), cache.k_off, cache.v_off)
+    want = ops.gqa_prefill(*args, kv_q8=q8)
+    for _ in range(20):
+        assert torch.equal(ops.gqa_prefill(*args, kv_q8=q8), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("ctx,rows,part", [(0, 300, 300), (4095, 1, 128), (3000, 33, 128), (0, 1100, 1100), (32704, 64, 1920)])
+def test_prefill_f32_is_finer_than_f16_operands(q8, ctx, rows, part):
+    """In the 2-norm of a head's row.  An operand whose lo half were left out would be off by up to 2^-12 of itself, 2^-13 rms.
+    What is there: scores, 2^-18 (48 truncated steps of |s| <= 5, half of 2^-23 each, of which softmax passes on the differences);
+    o, 2^-23 a step of 16 positions and operand half (two, q8_0 three)."""
+    from qwowl35_b200 import ops
+    n = ctx + rows
+    cache = Cache([n], q8, 5).fill([n], 6)
+    q, gt = some(rows, 1, torch.float32), some(rows, 2, torch.float32, 1.0)
+    out = ops.gqa_prefill(q, gt, ints(0, rows), ints(n), rows, n, cache.ptrs(), cache.k_off, cache.v_off, kv_q8=q8)
+    k, v = cache.sequence(0, n)
+    tol = 2.0 ** -18 + part / 16 * (3 if q8 else 2) * 2.0 ** -23
+    assert tol < 2.0 ** -14
+    for r in sorted({rows // 3, rows // 2, rows - 1}):
+        o = attend(q[r], gt[r], k, v, ctx + r + 1)[0]
+        err = (out[r].double().view(H, D) - o).norm(dim=-1) / o.norm(dim=-1)
+        assert float(err.max()) <= tol, (r, float(err.max()), tol)
+        # the bound tells: the plain form with q rounded to f16 is beyond it
+        half_q = attend(q[r].half(), gt[r], k, v, ctx + r + 1)[0]
+        assert float(((half_q - o).norm(dim=-1) / o.norm(dim=-1)).max()) > 2 * tol
+
+
+def test_append_refuses_sections_that_sum_to_32_by_wrapping():
+    """2^31 - 1 twice and 34 are 32 in 32 bits."""
+    with pytest.raises(_lib.Qw35Error, match="rotary sections"):
+        _lib.call("qw35_cuda_attn_append", *_append_args(sec=((1 << 31) - 1, (1 << 31) - 1, 34)))
