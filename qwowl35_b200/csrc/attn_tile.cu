@@ -60,12 +60,19 @@ constexpr float kShift = 7.0f, kSlack = 8.0f;  // log2: offset of P, growth of t
 constexpr float kNoScore = -3.0e38f;  // the maximum that a part leaves which has values but no finite score (an empty one: -infinity)
 
 // Positions that one O in TMEM sums up before the softmax warps put it away, adding it, rounded to nearest, to the row's sum
-// in the workspace, and the next product starts anew.  The tensor cores' adder truncates, which costs O about 2e-8 a step
-// of 16 positions and operand half.  f32 in one chain: 2.1e-5 (2-norm) after 8,192 positions, 8.7e-5 after 32,768 (q8_0
-// 17e-5), in pieces 6e-6 (10e-6), for which a prompt of 4,096 takes 317 us instead of 296, of 8,192 853 instead of 779, of
-// 32,768 13.0 ms instead of 12.4.  f16 has half the steps and 24e-5 of its own rounding, so its pieces are longer.  Parts no
-// longer than a piece take a kernel that cannot put away (AWAY false): f16 8192 tokens 435 us against 443 with one that can.
+// in the workspace, and the next product starts anew.  The tensor cores' adder truncates, step by step of 16 positions and
+// operand half.  f32 in one chain: off by 2.1e-5 (2-norm) after 8,192 positions, by 8.7e-5 after 32,768 (q8_0 17e-5); in
+// pieces 6e-6 (10e-6), with uncut() 3e-6 (4e-6).  For that a prompt of 4,096 takes 317 us instead of 296, of 8,192 853 instead
+// of 779, of 32,768 13.0 ms instead of 12.4; pieces of 1,024 (1.5e-6) took 64 tokens at 32,704 from 64 us to 70.  f16 has
+// half the steps and 24e-5 of its own rounding, so its pieces are longer.  Parts no longer than a piece take a kernel that
+// cannot put away (AWAY false): f16 8192 tokens 435 us against 443 with one that can.
 constexpr int kAwayF32 = 2048, kAwayF16 = 65536;
+
+// What a sum of `steps` steps (16 products each) is multiplied by for what the adder cut off: a step cuts 0 to 2^-23 of the
+// sum so far, 0.72 x 2^-24 on average over its mantissas, and the sum so far is half the sum on average.  That is the larger
+// part of the error: a 4096-token f32 prompt 2.7e-6 without, 1.4e-6 with, one token at 4096 1.25e-6 and 0.6e-6.
+constexpr float kCut = 4.3e-8f;
+__device__ __forceinline__ constexpr float uncut(int steps) { return 1.0f + 0.5f * kCut * (float)(steps + 1); }
 
 template <bool HL, bool Q8, bool PAIR>
 struct TileGeo {
@@ -90,6 +97,7 @@ struct TileGeo {
     static constexpr int PARTS = HL && Q8 ? 2 : 1;       // stages of a tile: values, or their hi and lo halves
     static constexpr uint32_t RING = NST * STAGE, SMEM = QB + RING;
     static constexpr uint32_t S0 = 256;                  // TMEM columns: O, then the S buffers, then (LO_TMEM) Q's lo half
+    static constexpr int STEPS = TK / 16 * (HL ? (Q8 ? 3 : 2) : 1);  // of a tile's product onto O
     static constexpr int AWAY = (HL ? kAwayF32 : kAwayF16) / TK;  // tiles after which O is put away
     // a lo half bound for TMEM passes through the last 64 KB of the ring
     static constexpr int FREE_AT_START = LO_TMEM ? (int)((RING - QBYTES) / STAGE) : NST;
@@ -956,7 +964,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
             }
         }
 
-        const float c = p.scale * kLog2e;
+        const float c = p.scale * kLog2e * uncut(AHD / 16);  // (lo products are too small to count)
         const int hi = real ? s.hi[tok] : 0x7fffffff, sk = real ? s.sk[tok] : 0, rs = real ? s.rs[tok] : 0;
         float m = -INFINITY, l = 0.0f;  // maximum in use; sum of this half's columns
         constexpr int CW = G::TK / 2, NB = CW / 32;
@@ -1002,6 +1010,8 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 float o[16];
                 tmem_ld16(tmem + lanes + b * 16, o);
                 if (real) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] *= uncut(G::AWAY * G::STEPS);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (!first) red_add4(to.piece(i), o + 4 * i);
@@ -1144,6 +1154,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 if (join && lane == 0) static_cast<float2 *>(p.ws)[head_row(r) * parts + s.part] = make_float2(fmaxf(rm, kNoScore), rl);
             }
         } else if (busy) {
+            const float whole = uncut((AWAY ? (n - 1) % G::AWAY + 1 : n) * G::STEPS);  // of O's last piece
             const float inv = join ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
             if (n > 0) {
                 if (AWAY && n > G::AWAY) {
@@ -1161,10 +1172,11 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             *reinterpret_cast<float4 *>(buf + row * BROW + b * 16 + 4 * i) =
-                                make_float4(fmaf(x[i].x, f, o[4 * i]) * inv, fmaf(x[i].y, f, o[4 * i + 1]) * inv,
-                                            fmaf(x[i].z, f, o[4 * i + 2]) * inv, fmaf(x[i].w, f, o[4 * i + 3]) * inv);
+                                make_float4(fmaf(x[i].x, f, o[4 * i] * whole) * inv, fmaf(x[i].y, f, o[4 * i + 1] * whole) * inv,
+                                            fmaf(x[i].z, f, o[4 * i + 2] * whole) * inv, fmaf(x[i].w, f, o[4 * i + 3] * whole) * inv);
                     }
                 } else {
+                    const float times = whole * inv;
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
                         float o[32];
@@ -1172,7 +1184,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
                             *reinterpret_cast<float4 *>(buf + row * BROW + grp * 128 + b * 32 + i) =
-                                make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+                                make_float4(o[i] * times, o[i + 1] * times, o[i + 2] * times, o[i + 3] * times);
                     }
                 }
             }

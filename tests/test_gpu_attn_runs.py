@@ -1305,3 +1305,24 @@ def test_append_refuses_sections_that_sum_to_32_by_wrapping():
     """2^31 - 1 twice and 34 are 32 in 32 bits."""
     with pytest.raises(_lib.Qw35Error, match="rotary sections"):
         _lib.call("qw35_cuda_attn_append", *_append_args(sec=((1 << 31) - 1, (1 << 31) - 1, 34)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("ctx,rows,part", [(0, 2000, 2000), (4095, 1, 128)])
+def test_prefill_f32_is_not_short_of_itself(q8, ctx, rows, part):
+    """A truncating adder leaves a sum of N steps short by 0 to N 2^-23 of it, some N / 2 steps of 0.72 x 2^-24, which is added
+    back: over many heads' rows, what is missing along the exact output is under a third of that (and 2^-21 of scores and gate)."""
+    from qwowl35_b200 import ops
+    n = ctx + rows
+    cache = Cache([n], q8, 5).fill([n], 6)
+    q, gt = some(rows, 1, torch.float32), some(rows, 2, torch.float32, 1.0)
+    out = ops.gqa_prefill(q, gt, ints(0, rows), ints(n), rows, n, cache.ptrs(), cache.k_off, cache.v_off, kv_q8=q8)
+    k, v = cache.sequence(0, n)
+    short = []
+    for r in range(max(0, rows - 120), rows, 7):
+        o = attend(q[r], gt[r], k, v, ctx + r + 1)[0]
+        short.append((((out[r].double().view(H, D) - o) * o).sum(-1) / (o * o).sum(-1)).mean())
+    steps = part / 16 * (3 if q8 else 2)
+    short = float(torch.stack(short).mean())
+    assert abs(short) <= 0.72 * 2.0 ** -24 * steps / 2 / 3 + 2.0 ** -21, (short, 0.72 * 2.0 ** -24 * steps / 2)
