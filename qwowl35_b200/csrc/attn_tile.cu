@@ -24,7 +24,8 @@
 //                 128 positions, each CTA holding half of it (cta_group::2): half
 //                 the L2 reads and twice the tiles in the ring.
 // f32 calls (HL) carry q and p as f16 hi + lo pairs, two products each, ~22
-// bits.  Q's lo half sits in TMEM for single CTAs, where 64-position S buffers
+// bits, and sums to 22: 0.6e-6 to 3e-6 of the output in the 2-norm, q8_0 up to 4e-6
+// (plain f32 0.4e-6 to 3.5e-6).  Q's lo half sits in TMEM for single CTAs, where 64-position S buffers
 // leave 128 columns and the ring keeps its size; for pairs, bound by the products
 // and so better off with 128 positions a product, beside Q (3 stages remain).
 // q8_0 values d * code (18 bits) then enter as hi + lo stages as well.  f16 calls
@@ -87,8 +88,9 @@ struct TileGeo {
     // f16 planes: four warps issue the copies; q8_0: eight convert, each an eighth of a stage (at six, with two
     // batches for some, a stage took 1.7 us and the products waited)
     static constexpr int LOADERS = Q8 ? 8 : 4;
-    // f16 over q8_0: 18 warps leave 96 registers a thread and softmax needs more (8192-token prompt 594 us with the
-    // split, 657 without); f32's smaller tiles do not, and the 14 warps over f16 planes have 128 (449 us; split 463)
+    // f16 over q8_0: 18 warps leave 96 registers a thread and softmax needs more (8192-token prompt 607 us with the split,
+    // 673 without).  f32 over q8_0 spills 50 to 160 bytes of a thread at 96 and has not been measured with a split.  The 14
+    // warps over f16 planes have 128 (449 us; split 463).
     static constexpr bool SPLIT = Q8 && !HL;
     static constexpr int THREADS = (SOFT_WARPS + LOADERS + (SPLIT ? 4 : 2)) * 32;  // and products, relay (two idle: whole groups of four)
     // registers a thread of softmax warps, loaders and the last four warps, within the launch's 96 a thread

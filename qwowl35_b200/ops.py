@@ -294,10 +294,11 @@ def gqa_decode_shared_workspace(n_seq: int, n_group: int, max_shared: int, max_o
 
 def gqa_decode_shared(q, gate, seq_len, group_off, shared_len, max_shared, max_own, chunk_ptrs, k_off, v_off, window=0,
                       sink=0, ws=None, out=None, kv_q8=False):
-    """gqa_decode for sequences that share prefixes, each prefix read once per group; [n, 4096] in q's type.
+    """gqa_decode for sequences that share prefixes, each read once for 32 sequences of a group; [n, 4096] in q's type.
 
     group_off [groups + 1], shared_len [groups] int32: sequences group_off[g]..group_off[g+1] agree on their first
-    shared_len[g] positions.  max_shared, max_own: upper bounds of shared_len and of seq_len - shared_len.
+    shared_len[g] positions, all of which the first one's table row holds.  max_shared, max_own: upper bounds of
+    shared_len and of seq_len - shared_len.
     """
     dev, dtype = _device_of(q), q.dtype
     n, groups, table = q.shape[0], shared_len.numel(), chunk_ptrs.shape
