@@ -164,7 +164,7 @@ int qw35_cuda_gqa_decode_noalloc(uint32_t n_seq, const float *q, const float *ga
 // streams, other graphs) need their own.  The size queries give 0 for sizes that
 // the call refuses or that leave it nothing to do; they allow for either dtype.
 //
-// Precision, in the 2-norm of an output row: f32 attention 0.6e-6 to 4e-6 (what
+// Precision, in the 2-norm of an output row: f32 attention 0.3e-6 to 4.3e-6 (what
 // f32 sums have, or up to four times that), at any length; f16 2e-4 to 4e-4, over
 // q8_0 planes 4e-4 to 8e-4 (a result rounded once: 2e-4).
 

@@ -24,9 +24,9 @@
 //                 128 positions, each CTA holding half of it (cta_group::2): half
 //                 the L2 reads and twice the tiles in the ring.
 // f32 calls (HL) carry q and p as f16 hi + lo pairs, two products each, ~22
-// bits, and sums to 22: 0.6e-6 to 3e-6 of the output in the 2-norm, q8_0 up to 4e-6
-// (plain f32 0.4e-6 to 3.5e-6).  Q's lo half sits in TMEM for single CTAs, where 64-position S buffers
-// leave 128 columns and the ring keeps its size; for pairs, bound by the products
+// bits: 0.3e-6 to 3e-6 of the output in the 2-norm, over q8_0 up to 4.3e-6 (plain
+// f32 0.4e-6 to 3.5e-6).  Q's lo half sits in TMEM for single CTAs, where
+// 64-position S buffers leave 128 columns and the ring keeps its size; for pairs, bound by the products
 // and so better off with 128 positions a product, beside Q (3 stages remain).
 // q8_0 values d * code (18 bits) then enter as hi + lo stages as well.  f16 calls
 // round p to f16 once, and q8_0 values once, the rounding their type implies.
@@ -63,17 +63,17 @@ constexpr float kNoScore = -3.0e38f;  // the maximum that a part leaves which ha
 // Positions that one O in TMEM sums up before the softmax warps put it away, adding it, rounded to nearest, to the row's sum
 // in the workspace, and the next product starts anew.  The tensor cores' adder truncates, step by step of 16 positions and
 // operand half.  f32 in one chain: off by 2.1e-5 (2-norm) after 8,192 positions, by 8.7e-5 after 32,768 (q8_0 17e-5); in
-// pieces 6e-6 (10e-6), with uncut() 3e-6 (4e-6).  For that a prompt of 4,096 takes 317 us instead of 296, of 8,192 853 instead
+// pieces 6e-6 (10e-6), with what was cut added back 3e-6 (4e-6).  For that a prompt of 4,096 takes 317 us instead of 296, of 8,192 853 instead
 // of 779, of 32,768 13.0 ms instead of 12.4; pieces of 1,024 (1.5e-6) took 64 tokens at 32,704 from 64 us to 70.  f16 has
 // half the steps and 24e-5 of its own rounding, so its pieces are longer.  Parts no longer than a piece take a kernel that
 // cannot put away (AWAY false): f16 8192 tokens 435 us against 443 with one that can.
 constexpr int kAwayF32 = 2048, kAwayF16 = 65536;
 
-// What a sum of `steps` steps (16 products each) is multiplied by for what the adder cut off: a step cuts 0 to 2^-23 of the
-// sum so far, 0.72 x 2^-24 on average over its mantissas, and the sum so far is half the sum on average.  That is the larger
-// part of the error: a 4096-token f32 prompt 2.7e-6 without, 1.4e-6 with, one token at 4096 1.25e-6 and 0.6e-6.
-constexpr float kCut = 4.3e-8f;
-__device__ __forceinline__ constexpr float uncut(int steps) { return 1.0f + 0.5f * kCut * (float)(steps + 1); }
+// A step of 16 products cuts 0 to 2^-23 of the sum so far, 0.72 x 2^-24 on average over mantissas, which is added back.  For
+// O the row's probabilities tell how far the sum had come at each step, and whether its products reach the sum's last place
+// at all (2^-24 each of it; the lo halves are 2^-11 of that): where they do not, nothing is cut.  A constant half of the
+// steps was off by 5.6e-6 behind a first position with all the weight.  A score is taken to be half there on average.
+constexpr float kCut = 4.3e-8f, kFelt = 0x1p-20f;
 
 template <bool HL, bool Q8, bool PAIR>
 struct TileGeo {
@@ -99,7 +99,7 @@ struct TileGeo {
     static constexpr int PARTS = HL && Q8 ? 2 : 1;       // stages of a tile: values, or their hi and lo halves
     static constexpr uint32_t RING = NST * STAGE, SMEM = QB + RING;
     static constexpr uint32_t S0 = 256;                  // TMEM columns: O, then the S buffers, then (LO_TMEM) Q's lo half
-    static constexpr int STEPS = TK / 16 * (HL ? (Q8 ? 3 : 2) : 1);  // of a tile's product onto O
+    static constexpr int STEPS = HL ? (Q8 ? 3 : 2) : 1;  // products of 16 positions onto O
     static constexpr int AWAY = (HL ? kAwayF32 : kAwayF16) / TK;  // tiles after which O is put away
     // a lo half bound for TMEM passes through the last 64 KB of the ring
     static constexpr int FREE_AT_START = LO_TMEM ? (int)((RING - QBYTES) / STAGE) : NST;
@@ -966,9 +966,11 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
             }
         }
 
-        const float c = p.scale * kLog2e * uncut(AHD / 16);  // (lo products are too small to count)
+        const float c = p.scale * kLog2e * (1.0f + kCut * (AHD / 16 + 1) / 2);  // (lo products are too small to count)
         const int hi = real ? s.hi[tok] : 0x7fffffff, sk = real ? s.sk[tok] : 0, rs = real ? s.rs[tok] : 0;
         float m = -INFINITY, l = 0.0f;  // maximum in use; sum of this half's columns
+        float way = 0.0f;               // sum of what l was at each step of this half's that O felt
+        float gone = 0.0f;              // sum of both halves up to where O was put away
         constexpr int CW = G::TK / 2, NB = CW / 32;
         const int parts = pl.ns + pl.ns_own;
         float *acc = reinterpret_cast<float *>(static_cast<float2 *>(p.ws) + (size_t)p.n_row * AH * parts);
@@ -990,10 +992,20 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
             return Place{acc + h * AHD + (full ? (r & 31) * 4 : b * 16), full ? parts * AHD : 8, full ? AHD / 2 : 4};
         };
         auto grown = [&]() { return ma == -INFINITY ? 1.0f : ex2((ma - m) * c); };  // (without a score so far: 0, or NaN and to stay so)
+        // l becomes both halves' sum; what O is multiplied by for what was cut off it.  (No warp is in a tile: both rows of ex
+        // are free.)
+        auto both_halves = [&]() {
+            s.ex[0][grp][row] = l;
+            s.ex[1][grp][row] = way;
+            named_sync(1 + quarter, 64);
+            l += s.ex[0][grp ^ 1][row];
+            way += s.ex[1][grp ^ 1][row];
+            return l > 0.0f ? 1.0f + kCut * 2 * __fdividef(way, l) : 1.0f;  // (at a step either half is as far)
+        };
         // O onto what was put away by additions in L2, which nothing waits for; no other thread has these values, so their
         // order is this one's.  Where a maximum grew since the last time, what is there takes its units first.
         auto put_away = [&](bool first) {
-            const float f = first || !real ? 1.0f : grown();
+            const float f = first || !real ? 1.0f : grown(), whole = both_halves();
             if (__any_sync(0xffffffffu, f != 1.0f)) {
 #pragma unroll 1
                 for (int b = grp * 8; b < grp * 8 + 8 && real; ++b) {
@@ -1013,7 +1025,7 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 tmem_ld16(tmem + lanes + b * 16, o);
                 if (real) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] *= uncut(G::AWAY * G::STEPS);
+                    for (int i = 0; i < 16; ++i) o[i] *= whole;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (!first) red_add4(to.piece(i), o + 4 * i);
@@ -1023,6 +1035,9 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 __syncwarp();
             }
             ma = m;
+            gone += l;
+            l = way = 0.0f;
+            named_sync(1 + quarter, 64);  // (ex has been read)
         };
         auto tile = [&](int j) {
             const uint32_t sb = tmem + lanes + G::S0 + (j & 1) * G::TK;
@@ -1073,6 +1088,8 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                         }
                     }
                     l *= alpha;
+                    way *= alpha;
+                    if (AWAY) gone *= alpha;
                     m = nm;
                 }
                 const float off = m == -INFINITY ? 0.0f : fmaf(m, c, -kShift);
@@ -1080,17 +1097,22 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 for (int b = 0; b < NB; ++b) {
                     uint32_t h[16];
                     [[maybe_unused]] uint32_t w[16];
-                    float l0 = 0.0f, l1 = 0.0f;
+                    float ls[2] = {0.0f, 0.0f};  // of the 16 positions of a step each
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float e0 = ex2(fmaf(__uint_as_float(u[b][2 * i]), c, -off));
                         const float e1 = ex2(fmaf(__uint_as_float(u[b][2 * i + 1]), c, -off));
-                        l0 += e0;
-                        l1 += e1;
+                        ls[i >> 3] += e0 + e1;
                         if constexpr (HL) split2(e0, e1, h[i], w[i]);
                         else h[i] = pack2(e0, e1);
                     }
-                    l += l0 + l1;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float at = fmaf(0.5f, ls[i], l);
+                        if (ls[i] > kFelt * l) way += at;
+                        if (G::STEPS > 1 && ls[i] > kFelt * 0x1p11f * l) way += (G::STEPS - 1) * at;
+                        l += ls[i];
+                    }
                     tmem_st16(sb + grp * (CW / 2) + b * 16, h);
                     if constexpr (HL) tmem_st16(sb + CW + grp * (CW / 2) + b * 16, w);
                 }
@@ -1140,11 +1162,8 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
         }
         float *buf = reinterpret_cast<float *>(smem);
         constexpr int BROW = AHD + 4;  // floats; 16-byte stores of 8 rows hit distinct banks
-        if (busy) {
-            s.ex[n & 1][grp][row] = l;
-            named_sync(1 + quarter, 64);
-            l += s.ex[n & 1][grp ^ 1][row];
-        }
+        const float whole = busy ? both_halves() : 1.0f;  // (of O's last piece)
+        if (AWAY) l += gone;
         if (n > 0 && *(volatile int *)&s.bad) {
             for (int r = warp; r < rows; r += SOFT_WARPS) {
                 float o[8], rm, rl;
@@ -1156,7 +1175,6 @@ __global__ void __launch_bounds__(TileGeo<HL, Q8, PAIR>::THREADS, 1) attn_tile_k
                 if (join && lane == 0) static_cast<float2 *>(p.ws)[head_row(r) * parts + s.part] = make_float2(fmaxf(rm, kNoScore), rl);
             }
         } else if (busy) {
-            const float whole = uncut((AWAY ? (n - 1) % G::AWAY + 1 : n) * G::STEPS);  // of O's last piece
             const float inv = join ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
             if (n > 0) {
                 if (AWAY && n > G::AWAY) {

@@ -1326,3 +1326,34 @@ def test_prefill_f32_is_not_short_of_itself(q8, ctx, rows, part):
     steps = part / 16 * (3 if q8 else 2)
     short = float(torch.stack(short).mean())
     assert abs(short) <= 0.72 * 2.0 ** -24 * steps / 2 / 3 + 2.0 ** -21, (short, 0.72 * 2.0 ** -24 * steps / 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("where,value,scale", [(None, 0, 12.0), (0, 32.0, 1.5), (0, 48.0, 1.5), (0, 64.0, 1.5), (0, 100.0, 1.5), (-1, 40.0, 1.5)])
+def test_prefill_f32_of_rows_that_lean_on_one_position(q8, where, value, scale):
+    """The first or the last position, or each row's own, outweighs the rest by e^8 to e^25.  How much of a sum is cut depends on
+    when it grew and on what still reaches its last place: what is added back follows that, and leaves at most 0.6 of the half
+    of all steps (0.72 x 2^-24 each) that rows without such a position lose, beside 2^-20 of the scores."""
+    from qwowl35_b200 import ops
+    n = 2000
+    cache = Cache([n], q8, 5).fill([n], 6)
+    q, gt = some(n, 1, torch.float32, scale), some(n, 2, torch.float32, 1.0)
+    if where is not None:
+        q[..., 3] = 4.0
+        pos = where % n
+        part = cache.rows()[int(cache.ids[0, pos // CH]), 0, :, pos % CH]
+        if q8:
+            part[:, 0, 2:] = 0
+            part[:, 0, 2 + 3] = 127
+            part[:, 0, :2] = torch.tensor([value / 127], dtype=torch.float16).view(torch.uint8).cuda()
+        else:
+            part[:, 3] = value
+    out = ops.gqa_prefill(q, gt, ints(0, n), ints(n), n, n, cache.ptrs(), cache.k_off, cache.v_off, kv_q8=q8)
+    k, v = cache.sequence(0, n)
+    errs = []
+    for r in range(n - 30, n, 3) if where != -1 else (n - 1,):
+        o = attend(q[r], gt[r], k, v, r + 1)[0]
+        errs.append(float((out[r].double().view(H, D) - o).norm() / o.norm()))
+    err = sum(errs) / len(errs)
+    assert err <= 0.6 * 0.72 * 2.0 ** -24 * n / 16 * (3 if q8 else 2) / 2 + 2.0 ** -20, err
