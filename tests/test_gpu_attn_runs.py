@@ -1357,3 +1357,38 @@ def test_prefill_f32_of_rows_that_lean_on_one_position(q8, where, value, scale):
         errs.append(float((out[r].double().view(H, D) - o).norm() / o.norm()))
     err = sum(errs) / len(errs)
     assert err <= 0.6 * 0.72 * 2.0 ** -24 * n / 16 * (3 if q8 else 2) / 2 + 2.0 ** -20, err
+
+
+@pytest.mark.gpu
+def test_captured_long_prompts_replay_on_two_streams():
+    """O of 5,000 positions leaves TMEM twice: the same bits in every replay, beside another graph with its own workspace, and right
+    for the lengths that stand in device memory."""
+    from qwowl35_b200 import ops
+    n, rows = 5000, 400
+    cache = Cache([n, n], False, 5).fill([n, n], 6)
+    q, gt = some(rows, 1, torch.float32), some(rows, 2, torch.float32, 1.0)
+    table = cache.ptrs()
+    lens = [ints(n), ints(n)]
+    off, outs = ints(0, rows), [torch.zeros(rows, H * D, device="cuda") for _ in range(2)]
+    ws = [ops.gqa_prefill_workspace(rows, 1, rows, n) for _ in range(2)]
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    tables = [table[i:i + 1].contiguous() for i in range(2)]
+    call = lambda i: ops.gqa_prefill(q, gt, off, lens[i], rows, n, tables[i], cache.k_off, cache.v_off, ws=ws[i], out=outs[i])  # noqa: E731
+    want = [call(i).clone() for i in range(2)]
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            call(i)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[i], want[i]) for i in range(2))
+    lens[1].copy_(ints(2100))
+    graphs[1].replay()
+    k, v = cache.sequence(1, 2100)
+    ref = [(r, *attend(q[r], gt[r], k, v, 2100 - rows + r + 1), 2100 - rows + r + 1) for r in (0, 63, 64, 347, 348, 349, rows - 1)]
+    check_rows(outs[1], ref, False, False)
+    assert _lib.lib().qw35_cuda_device_error() == 0
